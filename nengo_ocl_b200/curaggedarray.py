@@ -18,9 +18,9 @@ from io import StringIO
 
 import numpy as np
 
-from nengo_ocl_b200.raggedarray import RaggedArray
+from nengo_ocl_b200.raggedarray import _DTYPES, RaggedArray
 from nengo_ocl_b200.runtime import DeviceArray, to_device
-from nengo_ocl_b200.utils import equal_strides, is_iterable
+from nengo_ocl_b200.utils import as_dtype, bfloat16, equal_strides, is_iterable
 
 
 def to_host(queue, darray, dtype, start, shape, elemstrides):
@@ -145,7 +145,7 @@ class CUDARaggedArray:
     @buf.setter
     def buf(self, buf):
         buf = np.asarray(buf)
-        assert buf.dtype in (np.float32, np.int32)
+        assert buf.dtype in _DTYPES
         self.cl_buf = to_device(self.queue, buf)
 
     def __len__(self):
@@ -194,6 +194,9 @@ class CUDARaggedArray:
         start = int(self.starts[item])
         if m * n == 0:
             return
+        if self.dtype == bfloat16:
+            new_value = as_dtype(new_value, bfloat16)
+            new_value = new_value.reshape(m, n) if new_value.size == m * n else np.broadcast_to(new_value, (m, n))
         if (sm, sn) in [(1, m), (n, 1)] or equal_strides((sm, sn), (n, 1), (m, n)):
             # contiguous: one write
             if isinstance(new_value, np.ndarray):

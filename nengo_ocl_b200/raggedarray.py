@@ -2,7 +2,7 @@
 
 Same semantics as the reference's ``nengo_ocl/raggedarray.py:31-236``:
 
-* one flat ``buf`` (float32 or int32) plus five read-only int32 index arrays
+* one flat ``buf`` (float32 or int32; float16 / bfloat16 for the sequence operators) plus five read-only int32 index arrays
   ``starts / shape0s / shape1s / stride0s / stride1s`` (element units);
 * items are row-major by default (``stride0 = shape1``, ``stride1 = 1``);
 * ``align=True`` pads item starts to 16 / 4 / 1 elements depending on the
@@ -16,9 +16,9 @@ from io import StringIO
 
 import numpy as np
 
-from nengo_ocl_b200.utils import is_iterable, round_up
+from nengo_ocl_b200.utils import as_dtype, bfloat16, is_iterable, round_up
 
-_DTYPES = (np.dtype(np.float32), np.dtype(np.int32))
+_DTYPES = (np.dtype(np.float32), np.dtype(np.int32), np.dtype(np.float16), bfloat16)
 
 
 def _index_array(values):
@@ -64,7 +64,7 @@ class RaggedArray:
 
         buf = np.zeros(starts[-1] + sizes[-1], dtype=dtype)
         for a, s in zip(arrays, starts):
-            buf[s : s + a.size] = a.ravel()
+            buf[s : s + a.size] = as_dtype(a, dtype).ravel() if dtype == bfloat16 else a.ravel()
         self.buf = buf
         self.names = names
 

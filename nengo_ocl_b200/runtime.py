@@ -13,6 +13,7 @@ import weakref
 import numpy as np
 
 from nengo_ocl_b200 import _capi
+from nengo_ocl_b200.utils import bfloat16
 
 
 class Device:
@@ -79,12 +80,20 @@ def _free_stream(handle):
 
 
 class CommandQueue:
-    """An in-order CUDA stream."""
+    """An in-order CUDA stream.
 
-    def __init__(self, context=None, profiling=False):
+    ``stream``: an existing stream's handle (an int; 0 is the legacy default stream), e.g.
+    ``torch.cuda.current_stream().cuda_stream``.  Plans on the queue are then ordered with the other
+    work of that stream.  The stream must belong to the context's device and outlive the queue.
+    """
+
+    def __init__(self, context=None, profiling=False, stream=None):
         self.context = context if context is not None else create_some_context()
         self.device = self.context.devices[0]
         self.profiling = bool(profiling)
+        if stream is not None:
+            self.stream = int(stream)
+            return
         s = ctypes.c_void_p()
         _capi.call("nb2_stream_create", ctypes.byref(s))
         self.stream = s.value
@@ -132,7 +141,9 @@ class DeviceArray:
 
     @property
     def ctype(self):
-        return {"float32": "float", "int32": "int"}[self.dtype.name]
+        if self.dtype == bfloat16:
+            return "bfloat16"
+        return {"float32": "float", "int32": "int", "float16": "half"}[self.dtype.name]
 
     @property
     def start(self):
@@ -185,7 +196,7 @@ Array = DeviceArray
 
 
 def to_device(queue, array):
-    """Upload a host ndarray (float32 / int32) and return a DeviceArray."""
+    """Upload a host ndarray and return a DeviceArray."""
     array = np.ascontiguousarray(array)
     out = DeviceArray(queue, array.shape, array.dtype)
     out.set(array)

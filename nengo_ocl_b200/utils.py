@@ -7,6 +7,37 @@ its pyopencl / nengo imports.
 
 import numpy as np
 
+#: 16-bit floating point with float32's exponent.  numpy has no such type: values are stored as their
+#: upper 16 bits; ``to_bfloat16`` / ``from_bfloat16`` convert.
+bfloat16 = np.dtype([("bfloat16", "<u2")])
+
+
+def to_bfloat16(array):
+    """Round to the nearest bfloat16, ties to even; NaN stays NaN."""
+    array = np.asarray(array)
+    if array.dtype == bfloat16:
+        return array
+    bits = np.ascontiguousarray(array, dtype=np.float32).view(np.uint32)
+    rounded = ((bits.astype(np.uint64) + 0x7FFF + ((bits >> 16) & 1)) >> 16).astype(np.uint16)
+    nan = (bits & 0x7FFFFFFF) > 0x7F800000
+    rounded[nan] = (bits[nan] >> 16).astype(np.uint16) | 0x40
+    return rounded.view(bfloat16).reshape(array.shape)
+
+
+def from_bfloat16(array):
+    """The float32 values of a bfloat16 array (exact)."""
+    array = np.ascontiguousarray(array)
+    return (array.view(np.uint16).astype(np.uint32) << 16).view(np.float32).reshape(array.shape)
+
+
+def as_dtype(array, dtype):
+    """``np.asarray(array, dtype)``, for bfloat16 too."""
+    dtype = np.dtype(dtype)
+    if dtype == bfloat16:
+        return to_bfloat16(array)
+    array = np.asarray(array)
+    return (from_bfloat16(array) if array.dtype == bfloat16 else array).astype(dtype, copy=False)
+
 
 def is_iterable(obj):
     """True for lists/tuples/ranges and ndarrays with ndim > 0 (not scalars)."""
