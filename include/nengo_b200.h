@@ -441,6 +441,134 @@ int nb2_step_loop_wait_selftest(void* loop, void* stream);
 int nb2_step_loop_clear_status(void* loop, void* stream);
 int nb2_step_loop_status(void* loop, void* stream, int* status);
 
+/* ---- sequence operators ---------------------------------------------------
+ * Operators over sequences of rows (time steps or tokens) x channels, beside
+ * plan_linearfilter and plan_conv2d; the reference has no counterpart.  An
+ * array holds one block of rows per sequence; its place is in the int64 table
+ * [fields][n_seq] of the launch: field 0 = rows of the sequence, then start and
+ * row stride (elements) of each array in the order of the struct's comment, an
+ * absent array's fields being ignored.  units: int32 pairs (sequence, first
+ * row), each `unit_rows` rows.  dtype: the sequence arrays' element type;
+ * parameters, scan states and parameter gradients are float32.  vec: every
+ * sequence array allows 16-byte accesses (8 or 16 for the scan's states).
+ * `device` must be the current CUDA device of the calling thread. */
+#define NB2_F32 0
+#define NB2_F16 1
+#define NB2_BF16 2
+#define NB2_CONV_MAX_TAPS 8
+#define NB2_SCAN_MAX_STATES 128
+#define NB2_SCAN_KEEP 32 /* rows between two kept states of the scan */
+#define NB2_NORM_MAX_CHANNELS 32768
+
+/* y[t] = act(bias + sum_j w[c][j] x[t - taps + 1 + j]); rows before the first come from `state`
+ * (taps - 1 rows; NULL: zeros); new_state: the last taps - 1 rows (may be state itself).
+ * unit_rows >= taps - 1; a unit (sequence, 0) for every sequence, empty ones too.
+ * table: x, y, state, new_state */
+typedef struct {
+  int device, dtype, vec, n_seq, n_units, unit_rows, channels, taps, silu;
+  const int64_t* table;
+  const int* units;
+  const void* x;
+  void* y;
+  const float* w;    /* [channels][taps] */
+  const float* bias; /* NULL: none */
+  const void* state;
+  void* new_state;
+} nb2_causal_conv_args;
+int nb2_causal_conv(void* stream, const nb2_causal_conv_args* args);
+
+/* Backward of nb2_causal_conv: dx, dw, dbias, dstate from dy and dnew_state (NULL: zeros).
+ * part: float scratch [n_units][taps + 1][channels].  table: x, dy, dx, state, dstate, dnew_state */
+typedef struct {
+  int device, dtype, vec, n_seq, n_units, unit_rows, channels, taps, silu;
+  const int64_t* table;
+  const int* units;
+  const void *x, *dy;
+  void* dx;
+  const float *w, *bias;
+  const void* state;
+  void* dstate;
+  const void* dnew_state;
+  float *dw, *dbias, *part;
+} nb2_causal_conv_grad_args;
+int nb2_causal_conv_grad(void* stream, const nb2_causal_conv_grad_args* args);
+
+/* Per channel c of group g = c / (channels / groups), states n < n_states:
+ *   s = softplus(dt[t][c] + dt_bias[c]) (softplus != 0) or dt[t][c] + dt_bias[c]
+ *   h[n] = exp(s A[c][n]) h[n] + s x[t][c] B[t][g][n]
+ *   y[t][c] = (sum_n C[t][g][n] h[n] + D[c] x[t][c]) * (z ? z[t][c] sigmoid(z[t][c]) : 1)
+ * starting from state (channels x n_states rows per sequence; NULL: zeros), new_state receives the
+ * last h (may be state itself).  keep: float [blocks][channels][n_states] receives h before every
+ * NB2_SCAN_KEEP-th row, the blocks of sequence k beginning at field `first kept block`.
+ * table: x, dt, B, C, y, z, state, new_state, then (first kept block, -) */
+typedef struct {
+  int device, dtype, vec, state_vec, n_seq, channels, n_states, groups, softplus;
+  const int64_t* table;
+  const void *x, *dt, *B, *C;
+  void* y;
+  const void* z;
+  const float *A, *D, *dt_bias;
+  const float* state;
+  float* new_state;
+  float* keep;
+} nb2_selective_scan_args;
+int nb2_selective_scan(void* stream, const nb2_selective_scan_args* args);
+
+/* Backward of nb2_selective_scan from dy and dnew_state (NULL: zeros), with the states that the
+ * forward pass kept.  dz, dD, ddt_bias, dstate may be NULL.  part_bc: float scratch [channel tiles
+ * of a group][rows of all sequences][groups][2][n_states], part_a: float [n_seq][channels][n_states],
+ * part_d, part_s: float [n_seq][channels].
+ * table: x, dt, B, C, z, dy, dx, ddt, dB, dC, dz, dstate, dnew_state, then (first kept block, rows of
+ * the sequences before) */
+typedef struct {
+  int device, dtype, vec, state_vec, n_seq, channels, n_states, groups, softplus;
+  const int64_t* table;
+  const void *x, *dt, *B, *C, *z, *dy;
+  void *dx, *ddt, *dB, *dC, *dz;
+  const float *A, *D, *dt_bias, *keep;
+  float* dstate;
+  const float* dnew_state;
+  float *dA, *dD, *ddt_bias;
+  float *part_bc, *part_a, *part_d, *part_s;
+  int64_t total_rows;
+} nb2_selective_scan_grad_args;
+int nb2_selective_scan_grad(void* stream, const nb2_selective_scan_grad_args* args);
+/* channels that one block of the scan's backward pass covers (part_bc is sized by it) */
+int nb2_selective_scan_tile(int n_states);
+
+/* Row by row, silu(v) = v sigmoid(v):
+ *   u = gate_first ? x silu(gate) : x;   u = weight ? u rsqrt(mean over the group of u^2 + eps) weight : u
+ *   u = gate_first ? u : u silu(gate);   y = residual + scale u;   h = y rsqrt(mean(y^2) + eps) norm_weight
+ * (h from y before its rounding).  Absent: gate, residual, weight NULL leave their part out, scale NULL
+ * stands for scale_value, norm_weight NULL for ones; y or h may be NULL.
+ * table: x, y, h, gate, residual */
+typedef struct {
+  int device, dtype, vec, n_seq, n_units, unit_rows, channels, groups, gate_first;
+  float eps, scale_value;
+  const int64_t* table;
+  const int* units;
+  const void* x;
+  void *y, *h;
+  const void *gate, *residual;
+  const float *weight, *scale, *norm_weight;
+} nb2_residual_norm_args;
+int nb2_residual_norm(void* stream, const nb2_residual_norm_args* args);
+
+/* Backward of nb2_residual_norm from dy and dh (either may be NULL).  dgate, dresidual, dweight, dscale,
+ * dnorm_weight may be NULL.  part: float scratch [n_units][3][channels].
+ * table: x, gate, residual, dy, dh, dx, dgate, dresidual */
+typedef struct {
+  int device, dtype, vec, n_seq, n_units, unit_rows, channels, groups, gate_first;
+  float eps, scale_value;
+  const int64_t* table;
+  const int* units;
+  const void *x, *gate, *residual, *dy, *dh;
+  void *dx, *dgate, *dresidual;
+  const float *weight, *scale, *norm_weight;
+  float *dweight, *dscale, *dnorm_weight, *part;
+} nb2_residual_norm_grad_args;
+int nb2_residual_norm_grad(void* stream, const nb2_residual_norm_grad_args* args);
+
 #ifdef __cplusplus
 }
 #endif

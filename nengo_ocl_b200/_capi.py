@@ -9,7 +9,7 @@ use and raises ``RuntimeError`` if it has not been built
 import ctypes
 import os
 import re
-from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_size_t, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libnengo_b200.so")
@@ -36,6 +36,44 @@ class nb2_neuron_args(Structure):
         ("adaptive", c_int),
         ("fastlif", c_int),
     ]
+
+
+def _fields(ints, *pointers, tail=()):
+    return [(n, c_int) for n in ints.split()] + [(n, c_void_p) for p in pointers for n in p.split()] + list(tail)
+
+
+class nb2_causal_conv_args(Structure):
+    _fields_ = _fields("device dtype vec n_seq n_units unit_rows channels taps silu",
+                       "table units x y w bias state new_state")
+
+
+class nb2_causal_conv_grad_args(Structure):
+    _fields_ = _fields("device dtype vec n_seq n_units unit_rows channels taps silu",
+                       "table units x dy dx w bias state dstate dnew_state dw dbias part")
+
+
+class nb2_selective_scan_args(Structure):
+    _fields_ = _fields("device dtype vec state_vec n_seq channels n_states groups softplus",
+                       "table x dt B C y z A D dt_bias state new_state keep")
+
+
+class nb2_selective_scan_grad_args(Structure):
+    _fields_ = _fields("device dtype vec state_vec n_seq channels n_states groups softplus",
+                       "table x dt B C z dy dx ddt dB dC dz A D dt_bias keep dstate dnew_state dA dD ddt_bias",
+                       "part_bc part_a part_d part_s", tail=[("total_rows", c_int64)])
+
+
+_NORM_SCALARS = ([(n, c_int) for n in "device dtype vec n_seq n_units unit_rows channels groups gate_first".split()]
+                 + [("eps", c_float), ("scale_value", c_float)])
+
+
+class nb2_residual_norm_args(Structure):
+    _fields_ = _NORM_SCALARS + _fields("", "table units x y h gate residual weight scale norm_weight")
+
+
+class nb2_residual_norm_grad_args(Structure):
+    _fields_ = _NORM_SCALARS + _fields("", "table units x gate residual dy dh dx dgate dresidual weight scale",
+                                       "norm_weight dweight dscale dnorm_weight part")
 
 
 _P = c_void_p  # every device / host pointer crosses the boundary as void*
@@ -102,6 +140,13 @@ _SIGNATURES = {
     "nb2_pool2d": [_P, _P, _P] + [c_int] * 9,
     "nb2_ensemble_step": [_P, c_int, _P, c_int, _P, _P, _P, _P, _P, c_double],
     "nb2_direct": [_P, c_int, _P, c_int, c_int, _P, c_int, _P, _P, _P, _P, _P, _P],
+    "nb2_causal_conv": [_P, POINTER(nb2_causal_conv_args)],
+    "nb2_causal_conv_grad": [_P, POINTER(nb2_causal_conv_grad_args)],
+    "nb2_selective_scan": [_P, POINTER(nb2_selective_scan_args)],
+    "nb2_selective_scan_grad": [_P, POINTER(nb2_selective_scan_grad_args)],
+    "nb2_selective_scan_tile": [c_int],
+    "nb2_residual_norm": [_P, POINTER(nb2_residual_norm_args)],
+    "nb2_residual_norm_grad": [_P, POINTER(nb2_residual_norm_grad_args)],
     "nb2_step_loop_create": [POINTER(c_void_p)],
     "nb2_step_loop_destroy": [_P],
     "nb2_step_loop_finalize": [_P, c_int],

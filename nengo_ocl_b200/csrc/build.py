@@ -9,6 +9,7 @@ Python package, so the built library travels with the source tree.
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
@@ -34,6 +35,9 @@ UNITS = [
     ("nb2_fused.cu", ["-fmad=false"]),
     ("nb2_fused_stream.cu", ["-fmad=false"]),
     ("nb2_exchange.cu", []),
+    ("nb2_seq_conv.cu", []),
+    ("nb2_seq_scan.cu", []),
+    ("nb2_seq_norm.cu", []),
     # the persistent step loop reads what other CTAs wrote earlier in the same launch: global loads in L2 only
     ("nb2_step_loop.cu", ["-fmad=false", "-Xptxas", "-dlcm=cg"]),
     ("nb2_step_loop_single.cu", ["-fmad=false"]),
@@ -54,7 +58,7 @@ def build(force=False, verbose=False):
     headers.append(os.path.join(ROOT, "include", "nengo_b200.h"))
     headers.append(os.path.abspath(__file__))
     objs = []
-    rebuilt = False
+    todo = []
     for src, extra in UNITS:
         src_path = os.path.join(HERE, src)
         if not os.path.exists(src_path):
@@ -67,9 +71,11 @@ def build(force=False, verbose=False):
         if verbose:
             cmd += ["-Xptxas", "-v"]
             print(" ".join(cmd), flush=True)
-        subprocess.run(cmd, check=True)
-        rebuilt = True
-    if rebuilt or not os.path.exists(LIB) or force:
+        todo.append(cmd)
+    with ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+        for done in [pool.submit(subprocess.run, cmd, check=True) for cmd in todo]:
+            done.result()
+    if todo or not os.path.exists(LIB) or force:
         tmp = LIB + ".tmp"  # link beside the target and rename: a reader never sees a half-written library
         cmd = [nvcc, "-shared", "-o", tmp] + objs + ARCH + ["-Xcompiler", "-fPIC"]
         if verbose:

@@ -1,0 +1,89 @@
+// Shared by the sequence operators (causal convolution, selective scan, residual norm):
+// element types, vector loads and the layout of their tables.
+//
+// A sequence array holds one (rows x channels) block per sequence, rows `stride` elements
+// apart, channels next to each other.  The table of a launch is an int64 matrix
+// [fields][n_seq]: field 0 the number of rows, then (start, stride) of each array in
+// elements, so that offsets past 2^31 need no care in the kernels.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include "nb2_common.cuh"
+#include "../../include/nengo_b200.h"
+
+__device__ __forceinline__ float nb2_to_float(float v) { return v; }
+__device__ __forceinline__ float nb2_to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float nb2_to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T nb2_from_float(float v);
+template <>
+__device__ __forceinline__ float nb2_from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half nb2_from_float<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 nb2_from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// V elements next to each other: one 16-byte access when V * sizeof(T) == 16 (the caller has
+// checked the alignment), single elements otherwise.
+template <typename T, int V>
+struct SeqVec {
+  T e[V];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (V * sizeof(T) == 16)
+      *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(p);
+    else if constexpr (V * sizeof(T) == 8)
+      *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(p);
+    else
+#pragma unroll
+      for (int i = 0; i < V; ++i) e[i] = p[i];
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (V * sizeof(T) == 16)
+      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(e);
+    else if constexpr (V * sizeof(T) == 8)
+      *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(e);
+    else
+#pragma unroll
+      for (int i = 0; i < V; ++i) p[i] = e[i];
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = nb2_from_float<T>(0.0f);
+  }
+  __device__ __forceinline__ float operator[](int i) const { return nb2_to_float(e[i]); }
+};
+// (16-byte alignment of the register image, so that the casts above are allowed)
+template <typename T, int V>
+struct alignas(V * sizeof(T) >= 16 ? 16 : V * sizeof(T)) SeqVecA : SeqVec<T, V> {};
+
+__device__ __forceinline__ float nb2_sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+// d/dv [v sigmoid(v)]
+__device__ __forceinline__ float nb2_silu_slope(float v) {
+  const float s = nb2_sigmoid(v);
+  return s * (1.0f + v * (1.0f - s));
+}
+
+// The launch's device must be the calling thread's current one: the pointers belong to it.
+#define NB2_REQUIRE_DEVICE(ordinal)                                                     \
+  do {                                                                                  \
+    int dev__ = -1;                                                                     \
+    NB2_CUDA(cudaGetDevice(&dev__));                                                    \
+    NB2_REQUIRE(dev__ == (ordinal), "the plan's device is not the current CUDA device"); \
+  } while (0)
+
+#define NB2_SEQ_DTYPE(dtype, ...)                       \
+  do {                                                  \
+    if ((dtype) == NB2_F32) {                           \
+      using T = float;                                  \
+      __VA_ARGS__;                                      \
+    } else if ((dtype) == NB2_F16) {                    \
+      using T = __half;                                 \
+      __VA_ARGS__;                                      \
+    } else {                                            \
+      using T = __nv_bfloat16;                          \
+      __VA_ARGS__;                                      \
+    }                                                   \
+  } while (0)
+
+// out[i] = sum over p of part[p * n + i], p in order: the same result for every run
+cudaError_t nb2_seq_sum_parts(cudaStream_t s, const float* part, int64_t n_parts, int64_t n, float* out);
