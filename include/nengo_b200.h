@@ -457,7 +457,7 @@ int nb2_step_loop_status(void* loop, void* stream, int* status);
 #define NB2_BF16 2
 #define NB2_CONV_MAX_TAPS 8
 #define NB2_SCAN_MAX_STATES 128
-#define NB2_SCAN_KEEP 32 /* rows between two kept states of the scan */
+#define NB2_SCAN_KEEP 16 /* rows between two kept states of the scan */
 #define NB2_NORM_MAX_CHANNELS 32768
 
 /* y[t] = act(bias + sum_j w[c][j] x[t - taps + 1 + j]); rows before the first come from `state`
@@ -500,36 +500,47 @@ int nb2_causal_conv_grad(void* stream, const nb2_causal_conv_grad_args* args);
  * starting from state (channels x n_states rows per sequence; NULL: zeros), new_state receives the
  * last h (may be state itself).  keep: float [blocks][channels][n_states] receives h before every
  * NB2_SCAN_KEEP-th row, the blocks of sequence k beginning at field `first kept block`.
- * table: x, dt, B, C, y, z, state, new_state, then (first kept block, -) */
+ * tokens != 0: sequences of a few rows (any number is right), no units needed.  Else a block walks a unit
+ * (unit_rows a multiple of NB2_SCAN_KEEP, units of a sequence next to each other and in order, one for an
+ * empty sequence); with several units to a sequence ends (float [n_units][channels][n_states]) and sums
+ * (float [n_units][channels]) are scratch, with one both are NULL.
+ * rows_vec: x, dt, z allow 16-byte copies of a group's channels; vec: B and C allow 16-byte loads and
+ * n_states fills them; a_vec: A allows them.
+ * table: x, dt, B, C, y, z, state, new_state, then (first kept block, first unit) */
 typedef struct {
   int device, dtype, vec, state_vec, n_seq, channels, n_states, groups, softplus;
+  int tokens, rows_vec, a_vec, n_units, unit_rows;
   const int64_t* table;
+  const int* units;
   const void *x, *dt, *B, *C;
   void* y;
   const void* z;
   const float *A, *D, *dt_bias;
   const float* state;
   float* new_state;
-  float* keep;
+  float *keep, *ends, *sums;
 } nb2_selective_scan_args;
 int nb2_selective_scan(void* stream, const nb2_selective_scan_args* args);
 
 /* Backward of nb2_selective_scan from dy and dnew_state (NULL: zeros), with the states that the
- * forward pass kept.  dz, dD, ddt_bias, dstate may be NULL.  part_bc: float scratch [channel tiles
- * of a group][rows of all sequences][groups][2][n_states], part_a: float [n_seq][channels][n_states],
- * part_d, part_s: float [n_seq][channels].
+ * forward pass kept.  dz, dD, ddt_bias, dstate may be NULL.  Units, ends and sums as there (the units need
+ * not be the same); rows_vec also for dy.  part_bc: float scratch [channel tiles
+ * of a group][rows of all sequences][groups][2][n_states], part_a: float [n_units][channels][n_states],
+ * part_d, part_s: float [n_units][channels].
  * table: x, dt, B, C, z, dy, dx, ddt, dB, dC, dz, dstate, dnew_state, then (first kept block, rows of
- * the sequences before) */
+ * the sequences before), (first unit, -) */
 typedef struct {
   int device, dtype, vec, state_vec, n_seq, channels, n_states, groups, softplus;
+  int rows_vec, n_units, unit_rows;
   const int64_t* table;
+  const int* units;
   const void *x, *dt, *B, *C, *z, *dy;
   void *dx, *ddt, *dB, *dC, *dz;
   const float *A, *D, *dt_bias, *keep;
   float* dstate;
   const float* dnew_state;
   float *dA, *dD, *ddt_bias;
-  float *part_bc, *part_a, *part_d, *part_s;
+  float *part_bc, *part_a, *part_d, *part_s, *ends, *sums;
   int64_t total_rows;
 } nb2_selective_scan_grad_args;
 int nb2_selective_scan_grad(void* stream, const nb2_selective_scan_grad_args* args);

@@ -38,29 +38,32 @@ class nb2_neuron_args(Structure):
     ]
 
 
-def _fields(ints, *pointers, tail=()):
-    return [(n, c_int) for n in ints.split()] + [(n, c_void_p) for p in pointers for n in p.split()] + list(tail)
+def _fields(*ints, pointers, tail=()):
+    return ([(n, c_int) for names in ints for n in names.split()] + [(n, c_void_p) for n in pointers.split()]
+            + list(tail))
 
 
 class nb2_causal_conv_args(Structure):
     _fields_ = _fields("device dtype vec n_seq n_units unit_rows channels taps silu",
-                       "table units x y w bias state new_state")
+                       pointers="table units x y w bias state new_state")
 
 
 class nb2_causal_conv_grad_args(Structure):
     _fields_ = _fields("device dtype vec n_seq n_units unit_rows channels taps silu",
-                       "table units x dy dx w bias state dstate dnew_state dw dbias part")
+                       pointers="table units x dy dx w bias state dstate dnew_state dw dbias part")
 
 
 class nb2_selective_scan_args(Structure):
     _fields_ = _fields("device dtype vec state_vec n_seq channels n_states groups softplus",
-                       "table x dt B C y z A D dt_bias state new_state keep")
+                       "tokens rows_vec a_vec n_units unit_rows",
+                       pointers="table units x dt B C y z A D dt_bias state new_state keep ends sums")
 
 
 class nb2_selective_scan_grad_args(Structure):
     _fields_ = _fields("device dtype vec state_vec n_seq channels n_states groups softplus",
-                       "table x dt B C z dy dx ddt dB dC dz A D dt_bias keep dstate dnew_state dA dD ddt_bias",
-                       "part_bc part_a part_d part_s", tail=[("total_rows", c_int64)])
+                       "rows_vec n_units unit_rows",
+                       pointers="table units x dt B C z dy dx ddt dB dC dz A D dt_bias keep dstate dnew_state dA dD "
+                                "ddt_bias part_bc part_a part_d part_s ends sums", tail=[("total_rows", c_int64)])
 
 
 _NORM_SCALARS = ([(n, c_int) for n in "device dtype vec n_seq n_units unit_rows channels groups gate_first".split()]
@@ -68,12 +71,12 @@ _NORM_SCALARS = ([(n, c_int) for n in "device dtype vec n_seq n_units unit_rows 
 
 
 class nb2_residual_norm_args(Structure):
-    _fields_ = _NORM_SCALARS + _fields("", "table units x y h gate residual weight scale norm_weight")
+    _fields_ = _NORM_SCALARS + _fields(pointers="table units x y h gate residual weight scale norm_weight")
 
 
 class nb2_residual_norm_grad_args(Structure):
-    _fields_ = _NORM_SCALARS + _fields("", "table units x gate residual dy dh dx dgate dresidual weight scale",
-                                       "norm_weight dweight dscale dnorm_weight part")
+    _fields_ = _NORM_SCALARS + _fields(pointers="table units x gate residual dy dh dx dgate dresidual weight scale "
+                                                "norm_weight dweight dscale dnorm_weight part")
 
 
 _P = c_void_p  # every device / host pointer crosses the boundary as void*

@@ -62,6 +62,10 @@ __device__ __forceinline__ void nb2_pdl_enter() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// The same without the early trigger, for kernels that fill the GPU for long: the next kernel's blocks would
+// settle on the multiprocessors that become free first and stay there, unevenly, until this kernel ends.
+__device__ __forceinline__ void nb2_pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 template <typename... KArgs, typename... Args>
 static inline cudaError_t nb2_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
                                      Args... args) {

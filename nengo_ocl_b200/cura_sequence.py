@@ -30,8 +30,9 @@ from nengo_ocl_b200.utils import bfloat16, is_number
 _DTYPES = {np.dtype(np.float32): 0, np.dtype(np.float16): 1, bfloat16: 2}
 MAX_TAPS = 8            # NB2_CONV_MAX_TAPS
 MAX_STATES = 128        # NB2_SCAN_MAX_STATES
-KEEP_ROWS = 32          # NB2_SCAN_KEEP
+KEEP_ROWS = 16          # NB2_SCAN_KEEP
 MAX_NORM_CHANNELS = 32768  # NB2_NORM_MAX_CHANNELS
+TOKEN_ROWS = 4          # sequences of at most this many rows: the scan's token kernel
 
 
 # ---- argument checks -------------------------------------------------------------------------
@@ -341,6 +342,22 @@ def scan_tile(n_states):
     return 128 // lanes
 
 
+def _scan_units(a, args, tiles, want):
+    """Splits the sequences into units of rows.  A block walks a unit row after row, so a batch of few channels
+    or one long sequence is split over time until there are ``want`` blocks; that computes every row's
+    decay twice (once for the units' ends).  Returns the sequences' first units."""
+    longest, total = max(int(a.lengths.max()), 1), int(a.lengths.sum())
+    args.unit_rows = -(-longest // 32) * 32
+    if len(a.lengths) * tiles < want // 2 and longest > 128:
+        args.unit_rows = min(args.unit_rows, max(64, -(-total * tiles // (want * 32)) * 32))
+    units = np.maximum(-(-a.lengths // args.unit_rows), 1)
+    args.units, args.n_units = a.units(args.unit_rows)
+    if args.n_units > len(a.lengths):
+        args.ends = a.scratch(args.n_units * a.channels * args.n_states)
+        args.sums = a.scratch(args.n_units * a.channels)
+    return np.cumsum(units) - units
+
+
 def plan_selective_scan(queue, X, dt, A, B, C, Y, D=None, Z=None, dt_bias=None, softplus=False, state=None,
                         new_state=None, keep=False, tag=None):
     """The linear filter whose step size, input and output weights depend on the row::
@@ -368,16 +385,22 @@ def plan_selective_scan(queue, X, dt, A, B, C, Y, D=None, Z=None, dt_bias=None, 
         raise ValueError("B has %d columns: a multiple of the %d states that divides the channels is expected"
                          % (width, n))
     per = np.full(len(a.lengths), a.channels, np.int64)
-    args = _capi.nb2_selective_scan_args(
-        x=a.rows("X", X), dt=a.rows("dt", dt), B=a.rows("B", B, columns=width), C=a.rows("C", C, columns=width),
-        y=a.rows("Y", Y, written=True), z=a.rows("Z", Z, optional=True),
-        n_states=n, groups=groups, softplus=int(bool(softplus)), **a.common())
-    args.vec = int(a.aligned and n % 4 == 0)
+    args = _capi.nb2_selective_scan_args(x=a.rows("X", X), dt=a.rows("dt", dt), n_states=n, groups=groups,
+                                         softplus=int(bool(softplus)), **a.common())
+    each = 16 // a.dtype.itemsize  # elements of a 16-byte access
+    a.aligned, rows_aligned = True, a.aligned
+    args.B, args.C = a.rows("B", B, columns=width), a.rows("C", C, columns=width)
+    args.vec = int(a.aligned and n % each == 0)
+    args.y = a.rows("Y", Y, written=True)
+    a.aligned = rows_aligned
+    args.z = a.rows("Z", Z, optional=True)
+    args.rows_vec = int(a.aligned and (a.channels // groups) % each == 0)
     a.aligned = True
     args.state = a.rows("state", state, columns=n, lengths=per, dtype=np.float32, optional=True)
     args.new_state = a.rows("new_state", new_state, columns=n, lengths=per, dtype=np.float32, written=True, optional=True)
     args.state_vec = int(a.aligned and n % 4 == 0)
     args.A = a.param("A", A, (a.channels, n))
+    args.a_vec = int(args.A % 16 == 0)
     args.D = a.param("D", D, (a.channels,), optional=True)
     args.dt_bias = a.param("dt_bias", dt_bias, (a.channels,), optional=True)
     a.check_overlaps(in_place=("state", "new_state"))
@@ -386,10 +409,16 @@ def plan_selective_scan(queue, X, dt, A, B, C, Y, D=None, Z=None, dt_bias=None, 
     first = np.cumsum(blocks) - blocks
     if keep:
         args.keep = a.scratch(int(blocks.sum()) * a.channels * n)
-    args.table = a.table(first, np.zeros_like(first))
+    longest = int(a.lengths.max())
+    args.tokens = int(longest <= TOKEN_ROWS and not keep)
+    launches, first_unit = 1, np.arange(len(a.lengths))
+    if not args.tokens:
+        first_unit = _scan_units(a, args, groups * -(-(a.channels // groups) // scan_tile(n)), 148 * 4)
+        launches = 3 if args.ends else 1
+    args.table = a.table(first, first_unit)
     total = int(a.lengths.sum())
     plan = _make_plan(queue, "cura_selective_scan", "nb2_selective_scan", args, a.kept, len(a.lengths) * a.channels,
-                      1, tag, total * a.channels * (7 * n + 20), moved)
+                      launches, tag, total * a.channels * (7 * n + 20), moved)
     plan.sequence_args = dict(X=X, dt=dt, A=A, B=B, C=C, D=D, Z=Z, dt_bias=dt_bias, softplus=bool(softplus), state=state,
                               keep=args.keep, kept=a.kept, first=first, n=n, groups=groups)
     return plan
@@ -410,14 +439,18 @@ def plan_selective_scan_grad(queue, plan, dY, dX, ddt, dA, dB, dC, dD=None, dZ=N
     n, groups = f["n"], f["groups"]
     width = n * groups
     per = np.full(len(a.lengths), a.channels, np.int64)
-    args = _capi.nb2_selective_scan_grad_args(
-        x=a.rows("X", f["X"]), dt=a.rows("dt", f["dt"]), B=a.rows("B", f["B"], columns=width),
-        C=a.rows("C", f["C"], columns=width), z=a.rows("Z", f["Z"], optional=True), dy=a.rows("dY", dY),
-        dx=a.rows("dX", dX, written=True), ddt=a.rows("ddt", ddt, written=True),
-        dB=a.rows("dB", dB, columns=width, written=True), dC=a.rows("dC", dC, columns=width, written=True),
-        dz=a.rows("dZ", dZ, written=True, optional=True),
-        n_states=n, groups=groups, softplus=int(f["softplus"]), **a.common())
-    args.vec = int(a.aligned and n % 4 == 0)
+    args = _capi.nb2_selective_scan_grad_args(x=a.rows("X", f["X"]), dt=a.rows("dt", f["dt"]), n_states=n, groups=groups,
+                                              softplus=int(f["softplus"]), **a.common())
+    each = 16 // a.dtype.itemsize
+    a.aligned, rows_aligned = True, a.aligned
+    args.B, args.C = a.rows("B", f["B"], columns=width), a.rows("C", f["C"], columns=width)
+    args.vec = int(a.aligned and n % each == 0)
+    a.aligned = rows_aligned
+    args.z, args.dy = a.rows("Z", f["Z"], optional=True), a.rows("dY", dY)
+    args.rows_vec = int(a.aligned and (a.channels // groups) % each == 0)
+    args.dx, args.ddt = a.rows("dX", dX, written=True), a.rows("ddt", ddt, written=True)
+    args.dB, args.dC = a.rows("dB", dB, columns=width, written=True), a.rows("dC", dC, columns=width, written=True)
+    args.dz = a.rows("dZ", dZ, written=True, optional=True)
     a.aligned = True
     args.dstate = a.rows("dstate", dstate, columns=n, lengths=per, dtype=np.float32, written=True, optional=True)
     args.dnew_state = a.rows("dnew_state", dnew_state, columns=n, lengths=per, dtype=np.float32, optional=True)
@@ -434,14 +467,15 @@ def plan_selective_scan_grad(queue, plan, dY, dX, ddt, dA, dB, dC, dD=None, dZ=N
     a.kept.append(f["kept"])
     total = int(a.lengths.sum())
     args.total_rows = total
-    args.table = a.table(f["first"], np.cumsum(a.lengths) - a.lengths)
     tiles = -(-(a.channels // groups) // scan_tile(n))
+    first_unit = _scan_units(a, args, groups * tiles, 148 * 3)
+    args.table = a.table(f["first"], np.cumsum(a.lengths) - a.lengths, first_unit, np.zeros_like(first_unit))
     args.part_bc = a.scratch(tiles * total * 2 * width)
-    args.part_a = a.scratch(len(a.lengths) * a.channels * n)
-    args.part_d = a.scratch(len(a.lengths) * a.channels)
-    args.part_s = a.scratch(len(a.lengths) * a.channels)
+    args.part_a = a.scratch(args.n_units * a.channels * n)
+    args.part_d = a.scratch(args.n_units * a.channels)
+    args.part_s = a.scratch(args.n_units * a.channels)
     return _make_plan(queue, "cura_selective_scan_grad", "nb2_selective_scan_grad", args, a.kept,
-                      len(a.lengths) * a.channels, 5, tag, total * a.channels * (19 * n + 30), moved)
+                      len(a.lengths) * a.channels, 5 + 2 * bool(args.ends), tag, total * a.channels * (19 * n + 30), moved)
 
 
 # ---- norms around a block --------------------------------------------------------------------
