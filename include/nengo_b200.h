@@ -504,7 +504,7 @@ int nb2_causal_conv_grad(void* stream, const nb2_causal_conv_grad_args* args);
  * (unit_rows a multiple of NB2_SCAN_KEEP, units of a sequence next to each other and in order, one for an
  * empty sequence); with several units to a sequence ends (float [n_units][channels][n_states]) and sums
  * (float [n_units][channels]) are scratch, with one both are NULL.
- * rows_vec: x, dt, z allow 16-byte copies of a group's channels; vec: B and C allow 16-byte loads and
+ * rows_vec: x, dt, z, y allow 16-byte accesses to a group's channels; vec: B and C allow 16-byte loads and
  * n_states fills them; a_vec: A allows them.
  * table: x, dt, B, C, y, z, state, new_state, then (first kept block, first unit) */
 typedef struct {
@@ -524,7 +524,7 @@ int nb2_selective_scan(void* stream, const nb2_selective_scan_args* args);
 
 /* Backward of nb2_selective_scan from dy and dnew_state (NULL: zeros), with the states that the
  * forward pass kept.  dz, dD, ddt_bias, dstate may be NULL.  Units, ends and sums as there (the units need
- * not be the same); rows_vec also for dy.  part_bc: float scratch [channel tiles
+ * not be the same); rows_vec also for dy and the gradients.  part_bc: float scratch [channel tiles
  * of a group][rows of all sequences][groups][2][n_states], part_a: float [n_units][channels][n_states],
  * part_d, part_s: float [n_units][channels].
  * table: x, dt, B, C, z, dy, dx, ddt, dB, dC, dz, dstate, dnew_state, then (first kept block, rows of
@@ -544,8 +544,8 @@ typedef struct {
   int64_t total_rows;
 } nb2_selective_scan_grad_args;
 int nb2_selective_scan_grad(void* stream, const nb2_selective_scan_grad_args* args);
-/* channels that one block of the scan's backward pass covers (part_bc is sized by it) */
-int nb2_selective_scan_tile(int n_states);
+/* channels that one block of the scan covers (part_bc is sized by the backward pass's) */
+int nb2_selective_scan_tile(int n_states, int backward);
 
 /* Row by row, silu(v) = v sigmoid(v):
  *   u = gate_first ? x silu(gate) : x;   u = weight ? u rsqrt(mean over the group of u^2 + eps) weight : u

@@ -147,7 +147,7 @@ _SIGNATURES = {
     "nb2_causal_conv_grad": [_P, POINTER(nb2_causal_conv_grad_args)],
     "nb2_selective_scan": [_P, POINTER(nb2_selective_scan_args)],
     "nb2_selective_scan_grad": [_P, POINTER(nb2_selective_scan_grad_args)],
-    "nb2_selective_scan_tile": [c_int],
+    "nb2_selective_scan_tile": [c_int, c_int],
     "nb2_residual_norm": [_P, POINTER(nb2_residual_norm_args)],
     "nb2_residual_norm_grad": [_P, POINTER(nb2_residual_norm_grad_args)],
     "nb2_step_loop_create": [POINTER(c_void_p)],

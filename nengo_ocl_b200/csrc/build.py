@@ -37,6 +37,7 @@ UNITS = [
     ("nb2_exchange.cu", []),
     ("nb2_seq_conv.cu", []),
     ("nb2_seq_scan.cu", []),
+    ("nb2_seq_scan_grad.cu", []),
     ("nb2_seq_norm.cu", []),
     # the persistent step loop reads what other CTAs wrote earlier in the same launch: global loads in L2 only
     ("nb2_step_loop.cu", ["-fmad=false", "-Xptxas", "-dlcm=cg"]),

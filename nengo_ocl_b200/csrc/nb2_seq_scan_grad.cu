@@ -1,0 +1,441 @@
+// Backward pass of the selective scan.
+#include "nb2_seq_scan.cuh"
+
+// Backward.  With dp = dy silu(z), g[t] = C dp + a[t+1] g[t+1] (at the end: dnew_state):
+//   dz = dy p silu'(z), u = sum_n g B, dx = D dp + s u, ds = x u + sum_n g a h[t-1] A,
+//   ddt = ds softplus', dA = sum_t g a h[t-1] s, dB = sum_c g s x, dC = sum_c dp h, dstate = a[0] g[0].
+// A block walks its unit's NB2_SCAN_KEEP-row tiles from the last to the first: it recomputes a tile's decays
+// and states from the kept state into registers, then goes back through its rows.  Units as in the forward
+// pass, run through from the last: nb2_scan_grad_ends_kernel leaves the gradient that each would hand on if it
+// received zero.
+template <int S>
+struct ScanGradSmem {
+  static constexpr int R = NB2_SCAN_KEEP;
+  ScanRows<S, 1, R> ready;
+  float dp[R][ScanRows<S, 1, R>::kPitch];
+  alignas(16) float red[R][SCAN_WARPS][8 * S];  // dB, dC of a row: a warp's channels added
+};
+
+// Sums over the warp's channels (the lane bits S, 2 S ..) of eight values: transposed while there are values
+// to share, so lane bits choose which of them a lane ends up with (at, at + 1, .. of `kLeft`), then plain.
+template <int S>
+struct ScanChannelSum {
+  static constexpr int kStages = S == 32 ? 0 : S == 16 ? 1 : S == 8 ? 2 : 3;
+  static constexpr int kLeft = 8 >> kStages;
+  static __device__ __forceinline__ void sum(float (&v)[8], int lane) {
+    int w = S;
+#pragma unroll
+    for (int half = 4; half >= kLeft; half /= 2, w *= 2) {
+      const bool up = lane & w;
+#pragma unroll
+      for (int i = 0; i < half; ++i) {
+        const float keep = up ? v[i + half] : v[i], send = up ? v[i] : v[i + half];
+        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, w);
+      }
+    }
+#pragma unroll
+    for (int b = S << kStages; b < 32; b *= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], b);
+  }
+  static __device__ __forceinline__ int at(int lane) {
+    int i = 0;
+#pragma unroll
+    for (int q = 0; q < kStages; ++q)
+      if (lane & (S << q)) i += 4 >> q;
+    return i;
+  }
+  static __device__ __forceinline__ bool writes(int lane) { return lane < (S << kStages); }
+};
+
+template <typename T, int S, bool VEC>
+__global__ void __launch_bounds__(SCAN_THREADS) nb2_scan_grad_ends_kernel(const nb2_selective_scan_grad_args a) {
+  constexpr int R = NB2_SCAN_KEEP, RB = S < 4 ? S : 4;
+  constexpr int NA = 3;
+  using Stage = ScanStage<T, S, 1, R, NA>;
+  extern __shared__ __align__(16) char smem_raw[];
+  Stage* stages = reinterpret_cast<Stage*>(smem_raw);
+  ScanRows<S, 1, R>& ready = *reinterpret_cast<ScanRows<S, 1, R>*>(smem_raw + 2 * sizeof(Stage));
+  nb2_pdl_wait();
+  const ScanLane<S, 1> l(a.channels, a.groups, a.units);
+  const int n = a.n_states, c = l.channel(0);
+  const int64_t len = a.table[l.k], t0 = l.first, t1 = min(t0 + a.unit_rows, len), nk = a.n_seq;
+  if (t0 == 0) return;  // nothing comes before the first unit
+  const ScanPlace pt = scan_place(a.table, nk, 1, l.k), pb = scan_place(a.table, nk, 2, l.k),
+                  pc = scan_place(a.table, nk, 3, l.k), pz = scan_place(a.table, nk, 4, l.k),
+                  pdy = scan_place(a.table, nk, 5, l.k);
+  const T* dt = (const T*)a.dt + pt.start + t0 * pt.stride + l.c0;
+  const T* z = a.z ? (const T*)a.z + pz.start + t0 * pz.stride + l.c0 : nullptr;
+  const T* dy = (const T*)a.dy + pdy.start + t0 * pdy.stride + l.c0;
+  const T* B = (const T*)a.B + pb.start + t0 * pb.stride + (int64_t)l.group * n;
+  const T* C = (const T*)a.C + pc.start + t0 * pc.stride + (int64_t)l.group * n;
+  f32x2 A2[2], g[2] = {0, 0};
+  scan_rates(a.A + (int64_t)c * n, l.n0, n, A2);
+  const float bias = a.dt_bias ? a.dt_bias[c] : 0.0f;
+  const int j = l.j % RB, mine = l.in_block;
+  float total = 0.0f;
+  scan_clear_weights(stages, 2);
+  __syncthreads();
+  ScanWeights<VEC, T, S, R> weights;
+  ScanCopy<VEC, T, Stage> copy[NA];
+  auto fetch = [&](Stage& st, int64_t from, int rows) {
+    copy[0].load(st.in[0], dt + from * pt.stride, pt.stride, rows, l.width);
+    copy[1].load(st.in[1], dy + from * pdy.stride, pdy.stride, rows, l.width);
+    if (z)
+      copy[2].load(st.in[2], z + from * pz.stride, pz.stride, rows, l.width);
+    weights.load(B + from * pb.stride, pb.stride, C + from * pc.stride, pc.stride, n, rows);
+  };
+  auto arrive = [&](Stage& st) {
+    weights.store(st.bc, n);
+#pragma unroll
+    for (int i = 0; i < NA; ++i) copy[i].store(st.in[i]);
+  };
+  const int64_t all = t1 - t0, last = (all - 1) / R * R;
+  fetch(stages[0], last, (int)(all - last));
+  arrive(stages[0]);
+  int cur = 0;
+  for (int64_t tb = last; tb >= 0; tb -= R, cur ^= 1) {
+    const int rows = (int)min((int64_t)R, all - tb);
+    scan_cp_wait();
+    __syncthreads();
+    const Stage& st = stages[cur];
+    if (tb > 0) fetch(stages[cur ^ 1], tb - R, R);
+    scan_switch(a.softplus, [&](auto soft) {
+      scan_switch(z != nullptr, [&](auto gated) {
+#pragma unroll
+        for (int r0 = 0; r0 < R; r0 += RB) {
+          const int r = r0 + j;
+          float2 o;  // (s, dp)
+          o.x = nb2_to_float(st.in[0][r][mine]) + bias;
+          if (decltype(soft)::value) o.x = scan_softplus(o.x);
+          o.y = nb2_to_float(st.in[1][r][mine]);
+          if (decltype(gated)::value) {
+            const float zv = nb2_to_float(st.in[2][r][mine]);
+            o.y *= zv * nb2_sigmoid(zv);
+          }
+          if (r >= rows) o = make_float2(0.0f, 0.0f);
+          total += o.x;
+          if (RB == S || l.j < RB) ready.sx[r][mine] = o;
+        }
+      });
+    });
+    __syncwarp();
+#pragma unroll
+    for (int r = R - 1; r >= 0; --r) {
+      const float2 sd = ready.sx[r][mine];
+      const f32x2 s2 = pack2(sd.x, sd.x), d2 = pack2(sd.y, sd.y);
+      const ulonglong2 cw = *reinterpret_cast<const ulonglong2*>(&st.bc[r][1][l.n0]);
+      g[0] = mul2(exp2x2(mul2(s2, A2[0])), fma2(cw.x, d2, g[0]));
+      g[1] = mul2(exp2x2(mul2(s2, A2[1])), fma2(cw.y, d2, g[1]));
+    }
+    if (tb > 0) arrive(stages[cur ^ 1]);
+  }
+#pragma unroll
+  for (int w = 1; w < RB; w *= 2) total += __shfl_xor_sync(0xffffffffu, total, w);
+  if (l.valid(0)) {
+    float v[4];
+    unpack2(g[0], v[0], v[1]);
+    unpack2(g[1], v[2], v[3]);
+    const int64_t at = (int64_t)l.unit * a.channels + c;
+    scan_store4(a.ends + at * n, l.n0, n, n % 4 == 0, v);
+    if (l.j == 0) a.sums[at] = total;
+  }
+}
+
+template <typename T, int S, bool VEC>
+__global__ void __launch_bounds__(SCAN_THREADS) nb2_selective_scan_grad_kernel(const nb2_selective_scan_grad_args a) {
+  constexpr int R = NB2_SCAN_KEEP, RB = S < 4 ? S : 4;
+  constexpr int NA = 4;
+  using Stage = ScanStage<T, S, 1, R, NA>;
+  using Sum = ScanChannelSum<S>;
+  extern __shared__ __align__(16) char smem_raw[];
+  Stage* stages = reinterpret_cast<Stage*>(smem_raw);
+  ScanGradSmem<S>& sm = *reinterpret_cast<ScanGradSmem<S>*>(smem_raw + 2 * sizeof(Stage));
+  nb2_pdl_wait();
+  const ScanLane<S, 1> l(a.channels, a.groups, a.units);
+  const int n = a.n_states, c = l.channel(0), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t len = a.table[l.k], t0 = l.first, t1 = min(t0 + a.unit_rows, len), nk = a.n_seq;
+  const ScanPlace px = scan_place(a.table, nk, 0, l.k), pt = scan_place(a.table, nk, 1, l.k),
+                  pb = scan_place(a.table, nk, 2, l.k), pc = scan_place(a.table, nk, 3, l.k),
+                  pz = scan_place(a.table, nk, 4, l.k), pdy = scan_place(a.table, nk, 5, l.k),
+                  pdx = scan_place(a.table, nk, 6, l.k), pdt = scan_place(a.table, nk, 7, l.k),
+                  pdz = scan_place(a.table, nk, 10, l.k);
+  const T* x = (const T*)a.x + px.start + t0 * px.stride + l.c0;
+  const T* dt = (const T*)a.dt + pt.start + t0 * pt.stride + l.c0;
+  const T* z = a.z ? (const T*)a.z + pz.start + t0 * pz.stride + l.c0 : nullptr;
+  const T* dy = (const T*)a.dy + pdy.start + t0 * pdy.stride + l.c0;
+  const T* B = (const T*)a.B + pb.start + t0 * pb.stride + (int64_t)l.group * n;
+  const T* C = (const T*)a.C + pc.start + t0 * pc.stride + (int64_t)l.group * n;
+  T* dx = (T*)a.dx + pdx.start + t0 * pdx.stride + c;
+  T* ddt = (T*)a.ddt + pdt.start + t0 * pdt.stride + c;
+  T* dz = a.dz ? (T*)a.dz + pdz.start + t0 * pdz.stride + c : nullptr;
+  const float* keep = a.keep + ((a.table[27 * nk + l.k] + t0 / R) * a.channels + c) * n;
+  const int64_t row0 = a.table[28 * nk + l.k] + t0;
+  f32x2 A2[2], A[2], carry[2], dA[2] = {0, 0};
+  float v[4];
+  scan_rates(a.A + (int64_t)c * n, l.n0, n, A2);
+  scan_load4(a.A + (int64_t)c * n, l.n0, n, 0, v);
+  A[0] = pack2(v[0], v[1]);
+  A[1] = pack2(v[2], v[3]);
+#pragma unroll
+  for (int m = 0; m < 4; ++m) v[m] = 0.0f;
+  if (l.valid(0)) {
+    if (a.ends)
+      scan_load4(a.ends + ((int64_t)l.unit * a.channels + c) * n, l.n0, n, n % 4 == 0, v);
+    else if (a.dnew_state) {
+      const ScanPlace p = scan_place(a.table, nk, 12, l.k);
+      scan_load4(a.dnew_state + p.start + c * p.stride, l.n0, n, a.state_vec, v);
+    }
+  }
+  carry[0] = pack2(v[0], v[1]);
+  carry[1] = pack2(v[2], v[3]);
+  const float D = a.D ? a.D[c] : 0.0f, bias = a.dt_bias ? a.dt_bias[c] : 0.0f;
+  const int j = l.j % RB, mine = l.in_block;
+  const bool stores = l.valid(0) && l.j < RB;
+  float dD = 0.0f, dbias = 0.0f, h0[4];
+  scan_clear_weights(stages, 2);
+  __syncthreads();
+  ScanWeights<VEC, T, S, R> weights;
+  ScanCopy<VEC, T, Stage> copy[NA];
+  auto fetch = [&](Stage& st, int64_t from, int rows) {
+    copy[0].load(st.in[0], dt + from * pt.stride, pt.stride, rows, l.width);
+    copy[1].load(st.in[1], x + from * px.stride, px.stride, rows, l.width);
+    copy[2].load(st.in[2], dy + from * pdy.stride, pdy.stride, rows, l.width);
+    if (z)
+      copy[3].load(st.in[3], z + from * pz.stride, pz.stride, rows, l.width);
+    weights.load(B + from * pb.stride, pb.stride, C + from * pc.stride, pc.stride, n, rows);
+    scan_load4(keep + from / R * a.channels * n, l.n0, n, n % 4 == 0, h0);
+  };
+  auto arrive = [&](Stage& st) {
+    weights.store(st.bc, n);
+#pragma unroll
+    for (int i = 0; i < NA; ++i) copy[i].store(st.in[i]);
+  };
+  const int64_t all = t1 - t0, last = (all - 1) / R * R;
+  if (all > 0) {
+    fetch(stages[0], last, (int)(all - last));
+    arrive(stages[0]);
+  }
+  int cur = 0;
+  for (int64_t tb = all > 0 ? last : -1; tb >= 0; tb -= R, cur ^= 1) {
+    const int rows = (int)min((int64_t)R, all - tb);
+    scan_cp_wait();
+    __syncthreads();
+    const Stage& st = stages[cur];
+    const f32x2 start[2] = {pack2(h0[0], h0[1]), pack2(h0[2], h0[3])};
+    if (tb > 0) fetch(stages[cur ^ 1], tb - R, R);
+    scan_switch(a.softplus, [&](auto soft) {
+      scan_switch(z != nullptr, [&](auto gated) {
+#pragma unroll
+        for (int r0 = 0; r0 < R; r0 += RB) {
+          const int r = r0 + j;
+          float2 o;
+          o.x = nb2_to_float(st.in[0][r][mine]) + bias;
+          if (decltype(soft)::value) o.x = scan_softplus(o.x);
+          o.y = o.x * nb2_to_float(st.in[1][r][mine]);
+          float dp = nb2_to_float(st.in[2][r][mine]);
+          if (decltype(gated)::value) {
+            const float zv = nb2_to_float(st.in[3][r][mine]);
+            dp *= zv * nb2_sigmoid(zv);
+          }
+          if (r >= rows || !l.valid(0)) {  // (a lane without a channel adds nothing to dB, dC)
+            o = make_float2(0.0f, 0.0f);
+            dp = 0.0f;
+          }
+          if (RB == S || l.j < RB) {
+            sm.ready.sx[r][mine] = o;
+            sm.dp[r][mine] = dp;
+          }
+        }
+      });
+    });
+    __syncwarp();
+    f32x2 h[R][2], dec[R][2];
+    float out[R / RB], du[R / RB], de[R / RB];
+#pragma unroll
+    for (int r0 = 0; r0 < R; r0 += RB) {
+      float p[RB];
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        const int r = r0 + i;
+        const float2 sx = sm.ready.sx[r][mine];
+        const f32x2 s2 = pack2(sx.x, sx.x), x2 = pack2(sx.y, sx.y);
+        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&st.bc[r][0][l.n0]);
+        const ulonglong2 cw = *reinterpret_cast<const ulonglong2*>(&st.bc[r][1][l.n0]);
+        dec[r][0] = exp2x2(mul2(s2, A2[0]));
+        dec[r][1] = exp2x2(mul2(s2, A2[1]));
+        h[r][0] = fma2(dec[r][0], r ? h[r ? r - 1 : 0][0] : start[0], mul2(x2, b.x));
+        h[r][1] = fma2(dec[r][1], r ? h[r ? r - 1 : 0][1] : start[1], mul2(x2, b.y));
+        float lo, hi;
+        unpack2(fma2(cw.y, h[r][1], mul2(cw.x, h[r][0])), lo, hi);
+        p[i] = lo + hi;
+      }
+      out[r0 / RB] = 0.0f;
+      if (dz) {
+        float o = scan_transpose_sum<RB>(p, j);
+#pragma unroll
+        for (int w = RB; w < S; w *= 2) o += __shfl_xor_sync(0xffffffffu, o, w);
+        out[r0 / RB] = o;
+      }
+    }
+#pragma unroll
+    for (int r0 = R - RB; r0 >= 0; r0 -= RB) {
+      float pu[RB], pe[RB];
+#pragma unroll
+      for (int i = RB - 1; i >= 0; --i) {
+        const int r = r0 + i;
+        const float2 sx = sm.ready.sx[r][mine];
+        const float dp = sm.dp[r][mine];
+        const f32x2 s2 = pack2(sx.x, sx.x), x2 = pack2(sx.y, sx.y), d2 = pack2(dp, dp);
+        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&st.bc[r][0][l.n0]);
+        const ulonglong2 cw = *reinterpret_cast<const ulonglong2*>(&st.bc[r][1][l.n0]);
+        const f32x2 g0 = fma2(cw.x, d2, carry[0]), g1 = fma2(cw.y, d2, carry[1]);
+        carry[0] = mul2(g0, dec[r][0]);
+        carry[1] = mul2(g1, dec[r][1]);
+        const f32x2 q0 = mul2(carry[0], r ? h[r ? r - 1 : 0][0] : start[0]);
+        const f32x2 q1 = mul2(carry[1], r ? h[r ? r - 1 : 0][1] : start[1]);
+        dA[0] = fma2(q0, s2, dA[0]);
+        dA[1] = fma2(q1, s2, dA[1]);
+        float lo, hi;
+        unpack2(fma2(g1, b.y, mul2(g0, b.x)), lo, hi);
+        pu[i] = lo + hi;
+        unpack2(fma2(q1, A[1], mul2(q0, A[0])), lo, hi);
+        pe[i] = lo + hi;
+        float w[8];
+        unpack2(mul2(g0, x2), w[0], w[1]);
+        unpack2(mul2(g1, x2), w[2], w[3]);
+        unpack2(mul2(d2, h[r][0]), w[4], w[5]);
+        unpack2(mul2(d2, h[r][1]), w[6], w[7]);
+        Sum::sum(w, lane);
+        if (Sum::writes(lane)) {
+          const int at = Sum::at(lane);
+#pragma unroll
+          for (int m = 0; m < Sum::kLeft; ++m) sm.red[r][warp][((at + m) >> 2) * 4 * S + l.n0 + ((at + m) & 3)] = w[m];
+        }
+      }
+      float u = scan_transpose_sum<RB>(pu, j), e = scan_transpose_sum<RB>(pe, j);
+#pragma unroll
+      for (int w = RB; w < S; w *= 2) {
+        u += __shfl_xor_sync(0xffffffffu, u, w);
+        e += __shfl_xor_sync(0xffffffffu, e, w);
+      }
+      du[r0 / RB] = u;
+      de[r0 / RB] = e;
+    }
+    scan_switch(a.softplus, [&](auto soft) {
+      scan_switch(dz != nullptr, [&](auto gated) {
+#pragma unroll
+        for (int r0 = 0; r0 < R; r0 += RB) {
+          const int r = r0 + j;
+          const float raw = nb2_to_float(st.in[0][r][mine]) + bias, xv = nb2_to_float(st.in[1][r][mine]);
+          const float dp = sm.dp[r][mine], u = du[r0 / RB];
+          float ds = fmaf(xv, u, de[r0 / RB]), gz = 0.0f;
+          if (decltype(soft)::value) ds *= nb2_sigmoid(raw);
+          if (decltype(gated)::value)
+            gz = nb2_to_float(st.in[2][r][mine]) * fmaf(D, xv, out[r0 / RB]) * nb2_silu_slope(nb2_to_float(st.in[3][r][mine]));
+          if (r < rows && stores) {
+            dx[(tb + r) * pdx.stride] = nb2_from_float<T>(fmaf(D, dp, sm.ready.sx[r][mine].x * u));
+            ddt[(tb + r) * pdt.stride] = nb2_from_float<T>(ds);
+            if (decltype(gated)::value) dz[(tb + r) * pdz.stride] = nb2_from_float<T>(gz);
+            dD = fmaf(dp, xv, dD);
+            dbias += ds;
+          }
+        }
+      });
+    });
+    if (tb > 0) arrive(stages[cur ^ 1]);
+    __syncthreads();
+    // the block's share of dB and dC: warps in order
+    for (int i = tid; i < rows * 2 * n; i += SCAN_THREADS) {
+      const int r = i / (2 * n), m = i - r * 2 * n;
+      const int col = m < n ? m : 4 * S + m - n;
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < SCAN_WARPS; ++w) sum += sm.red[r][w][col];
+      a.part_bc[(((int64_t)l.tile * a.total_rows + row0 + tb + r) * a.groups + l.group) * 2 * n + m] = sum;
+    }
+  }
+#pragma unroll
+  for (int w = 1; w < RB; w *= 2) {
+    dD += __shfl_xor_sync(0xffffffffu, dD, w);
+    dbias += __shfl_xor_sync(0xffffffffu, dbias, w);
+  }
+  if (l.valid(0)) {
+    const int64_t at = (int64_t)l.unit * a.channels + c;
+    unpack2(dA[0], v[0], v[1]);
+    unpack2(dA[1], v[2], v[3]);
+    scan_store4(a.part_a + at * n, l.n0, n, 0, v);
+    if (l.j == 0) {
+      if (a.dD) a.part_d[at] = dD;
+      if (a.ddt_bias) a.part_s[at] = dbias;
+    }
+    if (a.dstate && t0 == 0) {
+      const ScanPlace p = scan_place(a.table, nk, 11, l.k);
+      unpack2(carry[0], v[0], v[1]);
+      unpack2(carry[1], v[2], v[3]);
+      scan_store4(a.dstate + p.start + c * p.stride, l.n0, n, a.state_vec, v);
+    }
+  }
+}
+
+// dB and dC of every row: the channel tiles' shares added in order.
+template <typename T>
+__global__ void __launch_bounds__(256) nb2_scan_grad_bc_kernel(const nb2_selective_scan_grad_args a, int tiles) {
+  nb2_pdl_enter();
+  const int n = a.n_states, wide = a.groups * 2 * n;
+  const int64_t all = a.total_rows * wide;
+  const int k = blockIdx.y;
+  const int64_t len = a.table[k], row0 = a.table[(size_t)28 * a.n_seq + k];
+  const ScanPlace pb = scan_place(a.table, a.n_seq, 8, k), pc = scan_place(a.table, a.n_seq, 9, k);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < len * wide; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / wide;
+    const int rest = (int)(i - r * wide), group = rest / (2 * n), m = rest - group * 2 * n;
+    float sum = 0.0f;
+    for (int u = 0; u < tiles; ++u) sum += a.part_bc[u * all + (row0 + r) * wide + rest];
+    if (m < n)
+      ((T*)a.dB)[pb.start + r * pb.stride + group * n + m] = nb2_from_float<T>(sum);
+    else
+      ((T*)a.dC)[pc.start + r * pc.stride + group * n + m - n] = nb2_from_float<T>(sum);
+  }
+}
+
+template <typename T, int S, bool VEC>
+static cudaError_t scan_grad_units(cudaStream_t s, const nb2_selective_scan_grad_args& a) {
+  constexpr int R = NB2_SCAN_KEEP;
+  const dim3 grid((unsigned)a.n_units * a.groups * scan_tiles(a.channels, a.groups, ScanLane<S, 1>::kBlock)), block(SCAN_THREADS);
+  if (a.ends) {
+    const size_t smem = 2 * sizeof(ScanStage<T, S, 1, R, 3>) + sizeof(ScanRows<S, 1, R>);
+    SCAN_TRY(scan_allow_smem(nb2_scan_grad_ends_kernel<T, S, VEC>, smem));
+    SCAN_TRY(nb2_launch(nb2_scan_grad_ends_kernel<T, S, VEC>, grid, block, smem, s, a));
+    SCAN_TRY(nb2_scan_join(s, ScanJoin{a.table, a.n_seq, a.n_states, a.unit_rows, 1, a.channels, 0, 29, a.A, a.dnew_state, 12, a.ends, a.sums}));
+  }
+  const size_t smem = 2 * sizeof(ScanStage<T, S, 1, R, 4>) + sizeof(ScanGradSmem<S>);
+  SCAN_TRY(scan_allow_smem(nb2_selective_scan_grad_kernel<T, S, VEC>, smem));
+  return nb2_launch(nb2_selective_scan_grad_kernel<T, S, VEC>, grid, block, smem, s, a);
+}
+
+template <typename T, int S>
+static cudaError_t scan_grad_launch(cudaStream_t s, const nb2_selective_scan_grad_args& a) {
+  return a.rows_vec && a.vec ? scan_grad_units<T, S, true>(s, a) : scan_grad_units<T, S, false>(s, a);
+}
+
+extern "C" int nb2_selective_scan_grad(void* stream, const nb2_selective_scan_grad_args* args) {
+  NB2_REQUIRE(args, "args");
+  const nb2_selective_scan_grad_args& a = *args;
+  if (int e = scan_check(a)) return e;
+  NB2_REQUIRE(a.dy && a.dx && a.ddt && a.dB && a.dC && a.dA && a.keep && a.part_bc && a.part_a, "null pointer");
+  NB2_REQUIRE((!a.dz || a.z) && (!a.dD || (a.D && a.part_d)) && (!a.ddt_bias || (a.dt_bias && a.part_s)), "gradients");
+  NB2_REQUIRE(a.n_seq <= 65535, "too many sequences");
+  if (int e = scan_check_units(a)) return e;
+  cudaStream_t s = nb2_stream(stream);
+  const int tiles = scan_tiles(a.channels, a.groups, SCAN_THREADS / scan_lanes(a.n_states));
+  NB2_SEQ_DTYPE(a.dtype, SCAN_BY_LANES(scan_lanes(a.n_states), scan_grad_launch));
+  if (a.total_rows > 0) {
+    const int64_t wide = (a.total_rows * a.groups * 2 * a.n_states + 255) / 256;
+    const int64_t per = (wide + a.n_seq - 1) / a.n_seq;
+    const dim3 grid((unsigned)(per < 8192 ? per : 8192), (unsigned)a.n_seq);
+    NB2_SEQ_DTYPE(a.dtype, NB2_CUDA(nb2_launch(nb2_scan_grad_bc_kernel<T>, grid, dim3(256), 0, s, a, tiles)));
+  }
+  NB2_CUDA(nb2_seq_sum_parts(s, a.part_a, a.n_units, (int64_t)a.channels * a.n_states, a.dA));
+  if (a.dD) NB2_CUDA(nb2_seq_sum_parts(s, a.part_d, a.n_units, a.channels, a.dD));
+  if (a.ddt_bias) NB2_CUDA(nb2_seq_sum_parts(s, a.part_s, a.n_units, a.channels, a.ddt_bias));
+  return NB2_OK;
+}

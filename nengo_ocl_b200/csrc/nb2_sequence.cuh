@@ -33,6 +33,8 @@ struct SeqVec {
       *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(p);
     else if constexpr (V * sizeof(T) == 8)
       *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(p);
+    else if constexpr (V > 1 && V * sizeof(T) == 4)
+      *reinterpret_cast<uint32_t*>(e) = *reinterpret_cast<const uint32_t*>(p);
     else
 #pragma unroll
       for (int i = 0; i < V; ++i) e[i] = p[i];
@@ -42,6 +44,8 @@ struct SeqVec {
       *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(e);
     else if constexpr (V * sizeof(T) == 8)
       *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(e);
+    else if constexpr (V > 1 && V * sizeof(T) == 4)
+      *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(e);
     else
 #pragma unroll
       for (int i = 0; i < V; ++i) p[i] = e[i];

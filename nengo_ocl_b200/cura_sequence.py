@@ -333,13 +333,13 @@ def plan_causal_conv_grad(queue, plan, dY, dX, dW, dbias=None, dstate=None, dnew
 
 
 # ---- selective state space scan --------------------------------------------------------------
-def scan_tile(n_states):
-    """Channels that one block of the scan covers (``nb2_selective_scan_tile``): four states to a lane,
-    as many lanes to a channel as the states need, 128 lanes to a block."""
+def scan_tile(n_states, backward=False):
+    """Channels that one block of the scan covers (``nb2_selective_scan_tile``): four states of two channels
+    (backward: of one) to a lane, as many lanes to a channel as the states need, 128 lanes to a block."""
     lanes = 1
     while 4 * lanes < n_states:
         lanes *= 2
-    return 128 // lanes
+    return 128 // lanes * (1 if backward else 2)
 
 
 def _scan_units(a, args, tiles, want):
@@ -391,9 +391,8 @@ def plan_selective_scan(queue, X, dt, A, B, C, Y, D=None, Z=None, dt_bias=None, 
     a.aligned, rows_aligned = True, a.aligned
     args.B, args.C = a.rows("B", B, columns=width), a.rows("C", C, columns=width)
     args.vec = int(a.aligned and n % each == 0)
-    args.y = a.rows("Y", Y, written=True)
     a.aligned = rows_aligned
-    args.z = a.rows("Z", Z, optional=True)
+    args.y, args.z = a.rows("Y", Y, written=True), a.rows("Z", Z, optional=True)
     args.rows_vec = int(a.aligned and (a.channels // groups) % each == 0)
     a.aligned = True
     args.state = a.rows("state", state, columns=n, lengths=per, dtype=np.float32, optional=True)
@@ -413,7 +412,7 @@ def plan_selective_scan(queue, X, dt, A, B, C, Y, D=None, Z=None, dt_bias=None, 
     args.tokens = int(longest <= TOKEN_ROWS and not keep)
     launches, first_unit = 1, np.arange(len(a.lengths))
     if not args.tokens:
-        first_unit = _scan_units(a, args, groups * -(-(a.channels // groups) // scan_tile(n)), 148 * 4)
+        first_unit = _scan_units(a, args, groups * -(-(a.channels // groups) // scan_tile(n)), 148 * 8)
         launches = 3 if args.ends else 1
     args.table = a.table(first, first_unit)
     total = int(a.lengths.sum())
@@ -447,10 +446,12 @@ def plan_selective_scan_grad(queue, plan, dY, dX, ddt, dA, dB, dC, dD=None, dZ=N
     args.vec = int(a.aligned and n % each == 0)
     a.aligned = rows_aligned
     args.z, args.dy = a.rows("Z", f["Z"], optional=True), a.rows("dY", dY)
-    args.rows_vec = int(a.aligned and (a.channels // groups) % each == 0)
     args.dx, args.ddt = a.rows("dX", dX, written=True), a.rows("ddt", ddt, written=True)
+    a.aligned, rows_aligned = True, a.aligned
     args.dB, args.dC = a.rows("dB", dB, columns=width, written=True), a.rows("dC", dC, columns=width, written=True)
+    a.aligned = rows_aligned
     args.dz = a.rows("dZ", dZ, written=True, optional=True)
+    args.rows_vec = int(a.aligned and (a.channels // groups) % each == 0)
     a.aligned = True
     args.dstate = a.rows("dstate", dstate, columns=n, lengths=per, dtype=np.float32, written=True, optional=True)
     args.dnew_state = a.rows("dnew_state", dnew_state, columns=n, lengths=per, dtype=np.float32, optional=True)
@@ -467,8 +468,8 @@ def plan_selective_scan_grad(queue, plan, dY, dX, ddt, dA, dB, dC, dD=None, dZ=N
     a.kept.append(f["kept"])
     total = int(a.lengths.sum())
     args.total_rows = total
-    tiles = -(-(a.channels // groups) // scan_tile(n))
-    first_unit = _scan_units(a, args, groups * tiles, 148 * 3)
+    tiles = -(-(a.channels // groups) // scan_tile(n, backward=True))
+    first_unit = _scan_units(a, args, groups * tiles, 148 * 8)
     args.table = a.table(f["first"], np.cumsum(a.lengths) - a.lengths, first_unit, np.zeros_like(first_unit))
     args.part_bc = a.scratch(tiles * total * 2 * width)
     args.part_a = a.scratch(args.n_units * a.channels * n)

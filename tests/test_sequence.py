@@ -360,8 +360,9 @@ def test_limits_agree_with_the_header():
         c["NB2_CONV_MAX_TAPS"], c["NB2_SCAN_MAX_STATES"], c["NB2_SCAN_KEEP"], c["NB2_NORM_MAX_CHANNELS"])
     assert list(seq._DTYPES.values()) == [c["NB2_F32"], c["NB2_F16"], c["NB2_BF16"]]
     for n in range(1, seq.MAX_STATES + 1):
-        assert _capi.lib().nb2_selective_scan_tile(n) == seq.scan_tile(n)
-    assert _capi.lib().nb2_selective_scan_tile(0) == -2
+        for backward in (0, 1):
+            assert _capi.lib().nb2_selective_scan_tile(n, backward) == seq.scan_tile(n, bool(backward))
+    assert _capi.lib().nb2_selective_scan_tile(0, 0) == -2
 
 
 def test_queue_over_an_existing_stream(fake_queue):
