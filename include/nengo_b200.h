@@ -550,11 +550,11 @@ int nb2_selective_scan_tile(int n_states, int backward);
 /* Row by row, silu(v) = v sigmoid(v):
  *   u = gate_first ? x silu(gate) : x;   u = weight ? u rsqrt(mean over the group of u^2 + eps) weight : u
  *   u = gate_first ? u : u silu(gate);   y = residual + scale u;   h = y rsqrt(mean(y^2) + eps) norm_weight
- * (h from y before its rounding).  Absent: gate, residual, weight NULL leave their part out, scale NULL
+ * (h from y before its rounding).  param_vec: the parameters allow 16-byte loads.  Absent: gate, residual, weight NULL leave their part out, scale NULL
  * stands for scale_value, norm_weight NULL for ones; y or h may be NULL.
  * table: x, y, h, gate, residual */
 typedef struct {
-  int device, dtype, vec, n_seq, n_units, unit_rows, channels, groups, gate_first;
+  int device, dtype, vec, n_seq, n_units, unit_rows, channels, groups, gate_first, param_vec;
   float eps, scale_value;
   const int64_t* table;
   const int* units;
@@ -566,10 +566,10 @@ typedef struct {
 int nb2_residual_norm(void* stream, const nb2_residual_norm_args* args);
 
 /* Backward of nb2_residual_norm from dy and dh (either may be NULL).  dgate, dresidual, dweight, dscale,
- * dnorm_weight may be NULL.  part: float scratch [n_units][3][channels].
+ * dnorm_weight may be NULL.  part: float scratch [n_units][2][channels].
  * table: x, gate, residual, dy, dh, dx, dgate, dresidual */
 typedef struct {
-  int device, dtype, vec, n_seq, n_units, unit_rows, channels, groups, gate_first;
+  int device, dtype, vec, n_seq, n_units, unit_rows, channels, groups, gate_first, param_vec;
   float eps, scale_value;
   const int64_t* table;
   const int* units;

@@ -66,7 +66,7 @@ class nb2_selective_scan_grad_args(Structure):
                                 "ddt_bias part_bc part_a part_d part_s ends sums", tail=[("total_rows", c_int64)])
 
 
-_NORM_SCALARS = ([(n, c_int) for n in "device dtype vec n_seq n_units unit_rows channels groups gate_first".split()]
+_NORM_SCALARS = ([(n, c_int) for n in "device dtype vec n_seq n_units unit_rows channels groups gate_first param_vec".split()]
                  + [("eps", c_float), ("scale_value", c_float)])
 
 

@@ -32,6 +32,7 @@ MAX_TAPS = 8            # NB2_CONV_MAX_TAPS
 MAX_STATES = 128        # NB2_SCAN_MAX_STATES
 KEEP_ROWS = 16          # NB2_SCAN_KEEP
 MAX_NORM_CHANNELS = 32768  # NB2_NORM_MAX_CHANNELS
+NORM_UNITS, NORM_GRAD_UNITS = 2, 1
 TOKEN_ROWS = 4          # sequences of at most this many rows: the scan's token kernel
 
 
@@ -519,10 +520,11 @@ def plan_residual_norm(queue, X, Y=None, H=None, gate=None, gate_first=True, res
     a.check_overlaps()
     moved = _nbytes(a.memory)
     args.vec = int(a.aligned and (a.channels // groups) % (16 // a.dtype.itemsize) == 0)
-    args.unit_rows = 1
+    args.param_vec = int(not any(p % 16 for p in (args.weight, args.scale, args.norm_weight) if p))
+    total = int(a.lengths.sum())
+    args.unit_rows = max(1, -(-total // (148 * NORM_UNITS)))
     args.table = a.table()
     args.units, args.n_units = a.units(args.unit_rows)
-    total = int(a.lengths.sum())
     plan = _make_plan(queue, "cura_residual_norm", "nb2_residual_norm", args, a.kept, total * a.channels, 1, tag,
                       total * a.channels * 16, moved)
     plan.sequence_args = dict(X=X, gate=gate, gate_first=gate_first, residual=residual, weight=weight, scale=scale,
@@ -564,10 +566,11 @@ def plan_residual_norm_grad(queue, plan, dX, dY=None, dH=None, dgate=None, dresi
     a.check_overlaps()
     moved = _nbytes(a.memory)
     args.vec = int(a.aligned and (a.channels // f["groups"]) % (16 // a.dtype.itemsize) == 0)
+    args.param_vec = int(not any(p % 16 for p in (args.weight, args.scale, args.norm_weight) if p))
     total = int(a.lengths.sum())
-    args.unit_rows = max(1, -(-total // (148 * 4)))
+    args.unit_rows = max(1, -(-total // (148 * NORM_GRAD_UNITS)))
     args.table = a.table()
     args.units, args.n_units = a.units(args.unit_rows)
-    args.part = a.scratch(args.n_units * 3 * a.channels)
+    args.part = a.scratch(args.n_units * 2 * a.channels)
     return _make_plan(queue, "cura_residual_norm_grad", "nb2_residual_norm_grad", args, a.kept, total * a.channels,
                       2, tag, total * a.channels * 40, moved)

@@ -356,7 +356,10 @@ NORMS = [  # chan, groups, pad, lead, gate, gate_first, residual, weight, scale,
     (9001, 1, 0, 0, True, True, True, True, True, True, True, True),
     (20000, 4, 0, 0, True, False, True, True, True, True, True, True),
     (32768, 1, 0, 0, True, True, True, True, True, True, True, True),
-    (32767, 1, 0, 0, True, True, True, True, True, True, False, True)]
+    (32767, 1, 0, 0, True, True, True, True, True, True, False, True),
+    (32766, 10922, 0, 0, True, False, True, True, True, True, True, True),
+    (1280, 5, 0, 0, True, True, True, True, True, True, True, True),
+    (3200, 100, 0, 0, False, True, True, True, 2.0, True, True, False)]
 
 
 @DTYPES
