@@ -39,6 +39,7 @@ UNITS = [
     ("nb2_seq_scan.cu", []),
     ("nb2_seq_scan_grad.cu", []),
     ("nb2_seq_norm.cu", []),
+    ("nb2_seq_norm_grad.cu", []),
     # the persistent step loop reads what other CTAs wrote earlier in the same launch: global loads in L2 only
     ("nb2_step_loop.cu", ["-fmad=false", "-Xptxas", "-dlcm=cg"]),
     ("nb2_step_loop_single.cu", ["-fmad=false"]),

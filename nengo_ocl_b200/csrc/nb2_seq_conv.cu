@@ -14,15 +14,27 @@ __device__ __forceinline__ ConvPlace conv_place(const int64_t* table, int n_seq,
   return {table[(size_t)(1 + 2 * array) * n_seq + k], table[(size_t)(2 + 2 * array) * n_seq + k]};
 }
 
+// The weights of a block's channels lie together in memory, V W of them to a thread: read in a row by all
+// threads and handed out through shared memory (an odd pitch keeps a warp's reads in different banks).
 template <int V, int W>
-__device__ __forceinline__ void conv_weights(const float* w, const float* bias, int c, float (&wr)[W][V], float (&b)[V]) {
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) wr[j][v] = w[(size_t)(c + v) * W + j];
-    b[v] = bias ? bias[c + v] : 0.0f;
+struct ConvWeights {
+  static constexpr int kEach = V * W, kPitch = kEach | 1, kFloats = CONV_THREADS * kPitch;
+  static __device__ __forceinline__ void stage(float* smem, const float* w, int c0, int channels) {
+    const int n = min(CONV_THREADS * V, channels - c0) * W;
+    const float* from = w + (size_t)c0 * W;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < n; i += CONV_THREADS) smem[i / kEach * kPitch + i % kEach] = from[i];
   }
-}
+  static __device__ __forceinline__ void get(const float* smem, const float* bias, int c, float (&wr)[W][V], float (&b)[V]) {
+    const float* mine = smem + threadIdx.x * kPitch;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) wr[j][v] = mine[v * W + j];
+      b[v] = bias ? bias[c + v] : 0.0f;
+    }
+  }
+};
 
 // The thread's V channels of row p of a sequence: the state's rows stand before row 0 (zeros without one).
 template <typename T, int V, int W>
@@ -35,12 +47,73 @@ __device__ __forceinline__ void conv_row(SeqVecA<T, V>& r, const T* x, int64_t x
     r.zero();
 }
 
+// The thread's V channels of the rows to come, kRows at a time: copied to shared memory while the ones
+// before them are worked on (a thread copies and reads its own channels only: no barrier).  Single elements, and a
+// unit of one group, are loaded straight into registers.
+template <typename T, int V, int kRows, int N>
+struct ConvRows {
+  static constexpr int kBytes = V * (int)sizeof(T), kAhead = 2;
+  static constexpr bool kAsync = kBytes == 16 || kBytes == 8;
+  const T* from[N];
+  int64_t stride[N];
+  int64_t end;  // rows from here on are zeros
+  bool async;
+  char* smem;
+  __host__ __device__ static constexpr int bytes() { return kAsync ? kAhead * kRows * N * CONV_THREADS * kBytes : 0; }
+  __device__ __forceinline__ char* slot(int group, int i, int q) const {
+    return smem + (((group % kAhead * kRows + i) * N + q) * CONV_THREADS + threadIdx.x) * kBytes;
+  }
+  __device__ __forceinline__ void ahead(int64_t t, int64_t stop, int group) const {
+    if constexpr (kAsync)
+      if (async) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+          if (t + i < stop)
+#pragma unroll
+            for (int q = 0; q < N; ++q) {
+              const unsigned to = (unsigned)__cvta_generic_to_shared(slot(group, i, q));
+              const T* row = from[q] + (t + i) * stride[q];
+              if constexpr (kBytes == 16)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(row) : "memory");
+              else
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(row) : "memory");
+            }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+  }
+  __device__ __forceinline__ void begin(int64_t t, int64_t stop) {
+    end = stop;
+    async = kAsync && stop - t > kRows;
+#pragma unroll
+    for (int g = 0; g < kAhead - 1; ++g) ahead(t + g * kRows, stop, g);
+  }
+  // group of rows t .. t + kRows - 1
+  __device__ __forceinline__ void get(int64_t t, int group, SeqVecA<T, V> (&r)[N][kRows]) const {
+    ahead(t + (kAhead - 1) * kRows, end, group + kAhead - 1);
+    if constexpr (kAsync)
+      if (async) asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        if (t + i >= end)
+          r[q][i].zero();
+        else if (kAsync && async)
+          r[q][i].load(reinterpret_cast<const T*>(slot(group, i, q)));
+        else
+          r[q][i].load(from[q] + (t + i) * stride[q]);
+      }
+  }
+};
+
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_kernel(const nb2_causal_conv_args a, int tiles) {
   nb2_pdl_enter();
+  extern __shared__ __align__(16) char smem[];
   const int unit = blockIdx.x / tiles;
-  const int c = ((blockIdx.x - unit * tiles) * CONV_THREADS + threadIdx.x) * V;
-  if (c >= a.channels) return;
+  const int c0 = (blockIdx.x - unit * tiles) * CONV_THREADS * V, c = c0 + threadIdx.x * V;
+  float* weights = reinterpret_cast<float*>(smem + ConvRows<T, V, 8, 1>::bytes());
+  ConvWeights<V, W>::stage(weights, a.w, c0, a.channels);
   const int k = a.units[2 * unit];
   const int64_t t0 = a.units[2 * unit + 1], len = a.table[k];
   const int64_t t1 = min(t0 + a.unit_rows, len);
@@ -54,8 +127,16 @@ __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_kernel(const nb2
     state = (const T*)a.state + p.start + c;
     ss = p.stride;
   }
+  constexpr int kRows = 8;
+  ConvRows<T, V, kRows, 1> in;
+  in.smem = smem;
+  in.from[0] = x;
+  in.stride[0] = px.stride;
+  if (c < a.channels) in.begin(t0, t1);
+  __syncthreads();
+  if (c >= a.channels) return;
   float w[W][V], b[V];
-  conv_weights<V, W>(a.w, a.bias, c, w, b);
+  ConvWeights<V, W>::get(weights, a.bias, c, w, b);
   float win[W][V];  // rows t - W + 1 .. t
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) {
@@ -64,20 +145,32 @@ __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_kernel(const nb2
 #pragma unroll
     for (int v = 0; v < V; ++v) win[j + 1][v] = r[v];
   }
-  for (int64_t t = t0; t < t1; ++t) {
-    SeqVecA<T, V> r, o;
-    r.load(x + t * px.stride);
+  int group = 0;
+  for (int64_t tb = t0; tb < t1; tb += kRows, ++group) {
+    const int rows = (int)min((int64_t)kRows, t1 - tb);
+    SeqVecA<T, V> r[1][kRows];
+    in.get(tb, group, r);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
+    for (int i = 0; i < kRows; ++i) {
+      if (i >= rows) break;
+      float out[V];
 #pragma unroll
-      for (int j = 0; j < W - 1; ++j) win[j][v] = win[j + 1][v];
-      win[W - 1][v] = r[v];
-      float s = b[v];
+      for (int v = 0; v < V; ++v) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) s = fmaf(w[j][v], win[j][v], s);
-      o.e[v] = nb2_from_float<T>(a.silu ? s * nb2_sigmoid(s) : s);
+        for (int j = 0; j < W - 1; ++j) win[j][v] = win[j + 1][v];
+        win[W - 1][v] = r[0][i][v];
+        float s = b[v];
+#pragma unroll
+        for (int j = 0; j < W; ++j) s = fmaf(w[j][v], win[j][v], s);
+        out[v] = s;
+      }
+      if (a.silu)
+#pragma unroll
+        for (int v = 0; v < V; ++v) out[v] *= nb2_sigmoid(out[v]);
+      SeqVecA<T, V> o;
+      o.put(out);
+      o.store(y + (tb + i) * py.stride);
     }
-    o.store(y + t * py.stride);
   }
   // The unit that read the old state writes the new one (so that the two may be the same rows): its
   // threads have read what they overwrite, and later rows of the old state are read before they are.
@@ -96,9 +189,11 @@ __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_kernel(const nb2
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_grad_kernel(const nb2_causal_conv_grad_args a, int tiles) {
   nb2_pdl_enter();
+  extern __shared__ __align__(16) char smem[];
   const int unit = blockIdx.x / tiles;
-  const int c = ((blockIdx.x - unit * tiles) * CONV_THREADS + threadIdx.x) * V;
-  if (c >= a.channels) return;
+  const int c0 = (blockIdx.x - unit * tiles) * CONV_THREADS * V, c = c0 + threadIdx.x * V;
+  float* weights = reinterpret_cast<float*>(smem + ConvRows<T, V, 4, 2>::bytes());
+  ConvWeights<V, W>::stage(weights, a.w, c0, a.channels);
   const int k = a.units[2 * unit];
   const int64_t t0 = a.units[2 * unit + 1], len = a.table[k];
   const int64_t t1 = min(t0 + a.unit_rows, len);
@@ -122,8 +217,16 @@ __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_grad_kernel(cons
     const ConvPlace p = conv_place(a.table, a.n_seq, 5, k);
     dnew = (const T*)a.dnew_state + p.start + c, ns = p.stride;
   }
+  constexpr int kRows = 4;
+  ConvRows<T, V, kRows, 2> in;
+  in.smem = smem;
+  in.from[0] = x, in.from[1] = dy;
+  in.stride[0] = px.stride, in.stride[1] = pdy.stride;
+  if (c < a.channels) in.begin(t0, min(t1 + W - 1, len));
+  __syncthreads();
+  if (c >= a.channels) return;
   float w[W][V], b[V], dw[W][V], db[V];
-  conv_weights<V, W>(a.w, a.bias, c, w, b);
+  ConvWeights<V, W>::get(weights, a.bias, c, w, b);
   float xw[W][V], gw[W][V];  // x and dpre of rows t - W + 1 .. t
 #pragma unroll
   for (int j = 0; j < W; ++j) {
@@ -137,61 +240,65 @@ __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_grad_kernel(cons
   for (int v = 0; v < V; ++v) db[v] = 0.0f;
   // The gradient of row p needs dpre of rows p .. p + W - 1, so the walk goes W - 1 rows past the unit;
   // the first unit also emits the W - 1 rows before the sequence, the state's gradient.
-  for (int64_t t = t0; t < t1 + W - 1; ++t) {
-    SeqVecA<T, V> rx, rg;
-    rx.zero();
-    rg.zero();
-    const bool in = t < len;
-    if (in) {
-      rx.load(x + t * px.stride);
-      rg.load(dy + t * pdy.stride);
-    }
-    const bool own = t < t1;
+  int group = 0;
+  for (int64_t tb = t0; tb < t1 + W - 1; tb += kRows, ++group) {
+    SeqVecA<T, V> r[2][kRows];
+    in.get(tb, group, r);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
+    for (int i = 0; i < kRows; ++i) {
+      const int64_t t = tb + i;
+      if (t >= t1 + W - 1) break;
+      float g[V];
 #pragma unroll
-      for (int j = 0; j < W - 1; ++j) xw[j][v] = xw[j + 1][v], gw[j][v] = gw[j + 1][v];
-      xw[W - 1][v] = rx[v];
-      float g = 0.0f;
-      if (in) {
-        g = rg[v];
-        if (a.silu) {
+      for (int v = 0; v < V; ++v) {
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) xw[j][v] = xw[j + 1][v], gw[j][v] = gw[j + 1][v];
+        xw[W - 1][v] = r[0][i][v];
+        g[v] = r[1][i][v];  // (zero past the sequence's end)
+      }
+      if (a.silu && t < len)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
           float s = b[v];
 #pragma unroll
           for (int j = 0; j < W; ++j) s = fmaf(w[j][v], xw[j][v], s);
-          g *= nb2_silu_slope(s);
+          g[v] *= nb2_silu_slope(s);
         }
-        if (own) {
-          db[v] += g;
 #pragma unroll
-          for (int j = 0; j < W; ++j) dw[j][v] = fmaf(g, xw[j][v], dw[j][v]);
+      for (int v = 0; v < V; ++v) gw[W - 1][v] = g[v];
+      if (t < t1)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          db[v] += g[v];
+#pragma unroll
+          for (int j = 0; j < W; ++j) dw[j][v] = fmaf(g[v], xw[j][v], dw[j][v]);
         }
+      const int64_t p = t - (W - 1);
+      if (p < t0 && !(t0 == 0 && dstate)) continue;
+      SeqVecA<T, V> add, o;
+      add.zero();
+      if (dnew && p >= len - (W - 1)) add.load(dnew + (p - len + (W - 1)) * ns);
+      float out[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float s = add[v];
+#pragma unroll
+        for (int j = 0; j < W; ++j) s = fmaf(w[W - 1 - j][v], gw[j][v], s);
+        out[v] = s;
       }
-      gw[W - 1][v] = g;
+      o.put(out);
+      if (p >= 0)
+        o.store(dx + p * pdx.stride);
+      else
+        o.store(dstate + (p + W - 1) * ds);
     }
-    const int64_t p = t - (W - 1);
-    if (p < t0 && !(t0 == 0 && dstate)) continue;
-    SeqVecA<T, V> add, o;
-    add.zero();
-    if (dnew && p >= len - (W - 1)) add.load(dnew + (p - len + (W - 1)) * ns);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float s = add[v];
-#pragma unroll
-      for (int j = 0; j < W; ++j) s = fmaf(w[W - 1 - j][v], gw[j][v], s);
-      o.e[v] = nb2_from_float<T>(s);
-    }
-    if (p >= 0)
-      o.store(dx + p * pdx.stride);
-    else
-      o.store(dstate + (p + W - 1) * ds);
   }
   float* part = a.part + (size_t)unit * (W + 1) * a.channels + c;
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) part[(size_t)j * a.channels + v] = dw[j][v];
-    part[(size_t)W * a.channels + v] = db[v];
+  for (int j = 0; j <= W; ++j) {
+    SeqVecA<float, V> o;
+    o.put(j < W ? dw[j < W ? j : 0] : db);
+    o.store(part + (size_t)j * a.channels);
   }
 }
 
@@ -248,15 +355,24 @@ cudaError_t nb2_seq_sum_parts(cudaStream_t s, const float* part, int64_t n_parts
                     n_parts, n, out);
 }
 
+template <typename K, typename A>
+static cudaError_t conv_run(K kernel, dim3 grid, int smem, cudaStream_t s, const A& a, int tiles) {
+  if (smem > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+  }
+  return nb2_launch(kernel, grid, dim3(CONV_THREADS), smem, s, a, tiles);
+}
+
 template <typename T, int V>
 static cudaError_t conv_launch(cudaStream_t s, const nb2_causal_conv_args& a) {
   const int tiles = (a.channels + V * CONV_THREADS - 1) / (V * CONV_THREADS);
-  const dim3 grid((unsigned)a.n_units * tiles), block(CONV_THREADS);
+  const dim3 grid((unsigned)a.n_units * tiles);
 #define NB2_CASE(W) \
-  case W: return nb2_launch(nb2_causal_conv_kernel<T, V, W>, grid, block, 0, s, a, tiles)
+  case W: return conv_run(nb2_causal_conv_kernel<T, V, W>, grid, ConvRows<T, V, 8, 1>::bytes() + 4 * ConvWeights<V, W>::kFloats, s, a, tiles)
   switch (a.taps) {
     NB2_CASE(1); NB2_CASE(2); NB2_CASE(3); NB2_CASE(4); NB2_CASE(5); NB2_CASE(6); NB2_CASE(7);
-    default: return nb2_launch(nb2_causal_conv_kernel<T, V, 8>, grid, block, 0, s, a, tiles);
+    default: return conv_run(nb2_causal_conv_kernel<T, V, 8>, grid, ConvRows<T, V, 8, 1>::bytes() + 4 * ConvWeights<V, 8>::kFloats, s, a, tiles);
   }
 #undef NB2_CASE
 }
@@ -264,12 +380,12 @@ static cudaError_t conv_launch(cudaStream_t s, const nb2_causal_conv_args& a) {
 template <typename T, int V>
 static cudaError_t conv_grad_launch(cudaStream_t s, const nb2_causal_conv_grad_args& a) {
   const int tiles = (a.channels + V * CONV_THREADS - 1) / (V * CONV_THREADS);
-  const dim3 grid((unsigned)a.n_units * tiles), block(CONV_THREADS);
+  const dim3 grid((unsigned)a.n_units * tiles);
 #define NB2_CASE(W) \
-  case W: return nb2_launch(nb2_causal_conv_grad_kernel<T, V, W>, grid, block, 0, s, a, tiles)
+  case W: return conv_run(nb2_causal_conv_grad_kernel<T, V, W>, grid, ConvRows<T, V, 4, 2>::bytes() + 4 * ConvWeights<V, W>::kFloats, s, a, tiles)
   switch (a.taps) {
     NB2_CASE(1); NB2_CASE(2); NB2_CASE(3); NB2_CASE(4); NB2_CASE(5); NB2_CASE(6); NB2_CASE(7);
-    default: return nb2_launch(nb2_causal_conv_grad_kernel<T, V, 8>, grid, block, 0, s, a, tiles);
+    default: return conv_run(nb2_causal_conv_grad_kernel<T, V, 8>, grid, ConvRows<T, V, 4, 2>::bytes() + 4 * ConvWeights<V, 8>::kFloats, s, a, tiles);
   }
 #undef NB2_CASE
 }
@@ -300,7 +416,8 @@ extern "C" int nb2_causal_conv_grad(void* stream, const nb2_causal_conv_grad_arg
   const nb2_causal_conv_grad_args& a = *args;
   if (int e = conv_check(a)) return e;
   NB2_REQUIRE(a.dy && a.dx && a.dw && a.part, "null pointer");
-  NB2_SEQ_DTYPE(a.dtype, if (a.vec) NB2_CUDA((conv_grad_launch<T, 16 / sizeof(T)>(nb2_stream(stream), a)));
+  // four channels to a thread whatever the type: the two windows, the weights and their sums are 16 W registers
+  NB2_SEQ_DTYPE(a.dtype, if (a.vec) NB2_CUDA((conv_grad_launch<T, 4>(nb2_stream(stream), a)));
                 else NB2_CUDA((conv_grad_launch<T, 1>(nb2_stream(stream), a))));
   const int64_t n = (int64_t)(a.taps + 1) * a.channels;
   NB2_CUDA(nb2_launch(nb2_conv_grad_sum_kernel, dim3((unsigned)((n + 31) / 32)), dim3(256), 0, nb2_stream(stream), a.part,

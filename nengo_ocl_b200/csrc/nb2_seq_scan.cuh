@@ -208,8 +208,7 @@ template <bool VEC, typename T, int P>
 __device__ __forceinline__ void scan_put(T* to, const float (&v)[P], int valid) {
   if constexpr (VEC) {
     SeqVecA<T, P> r;
-#pragma unroll
-    for (int p = 0; p < P; ++p) r.e[p] = nb2_from_float<T>(v[p]);
+    r.put(v);
     if (valid > 0) r.store(to);
   } else {
 #pragma unroll

@@ -23,11 +23,20 @@ __device__ __forceinline__ __half nb2_from_float<__half>(float v) { return __flo
 template <>
 __device__ __forceinline__ __nv_bfloat16 nb2_from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+template <typename T>
+struct IsHalf {
+  static constexpr bool value = false;
+};
+template <>
+struct IsHalf<__half> {
+  static constexpr bool value = true;
+};
+
 // V elements next to each other: one 16-byte access when V * sizeof(T) == 16 (the caller has
 // checked the alignment), single elements otherwise.
 template <typename T, int V>
-struct SeqVec {
-  T e[V];
+struct SeqVecA {
+  alignas(V * sizeof(T) >= 16 ? 16 : V * sizeof(T)) T e[V];
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (V * sizeof(T) == 16)
       *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(p);
@@ -54,12 +63,31 @@ struct SeqVec {
 #pragma unroll
     for (int i = 0; i < V; ++i) e[i] = nb2_from_float<T>(0.0f);
   }
-  __device__ __forceinline__ float operator[](int i) const { return nb2_to_float(e[i]); }
+  // (a pair of bfloat16 is two shifts of its word)
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (V > 1 && sizeof(T) == 2 && !IsHalf<T>::value) {
+      const uint32_t w = reinterpret_cast<const uint32_t*>(e)[i >> 1];
+      return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+    } else {
+      return nb2_to_float(e[i]);
+    }
+  }
+  // rounds v, two to a conversion where the type has one
+  __device__ __forceinline__ void put(const float (&v)[V]) {
+    if constexpr (V > 1 && sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < V; i += 2) {
+        if constexpr (IsHalf<T>::value)
+          reinterpret_cast<__half2*>(e)[i >> 1] = __floats2half2_rn(v[i], v[i + 1]);
+        else
+          reinterpret_cast<__nv_bfloat162*>(e)[i >> 1] = __floats2bfloat162_rn(v[i], v[i + 1]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) e[i] = nb2_from_float<T>(v[i]);
+    }
+  }
 };
-// (16-byte alignment of the register image, so that the casts above are allowed)
-template <typename T, int V>
-struct alignas(V * sizeof(T) >= 16 ? 16 : V * sizeof(T)) SeqVecA : SeqVec<T, V> {};
-
 __device__ __forceinline__ float nb2_sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
 // d/dv [v sigmoid(v)]
 __device__ __forceinline__ float nb2_silu_slope(float v) {
