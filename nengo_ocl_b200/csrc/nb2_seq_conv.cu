@@ -106,7 +106,7 @@ struct ConvRows {
   }
 };
 
-template <typename T, int V, int W>
+template <typename T, int V, int W, bool SILU>
 __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_kernel(const nb2_causal_conv_args a, int tiles) {
   nb2_pdl_enter();
   extern __shared__ __align__(16) char smem[];
@@ -150,9 +150,9 @@ __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_kernel(const nb2
     const int rows = (int)min((int64_t)kRows, t1 - tb);
     SeqVecA<T, V> r[1][kRows];
     in.get(tb, group, r);
+    // (no way out of this loop: the window then moves by renaming registers)
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      if (i >= rows) break;
       float out[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
@@ -164,12 +164,12 @@ __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_kernel(const nb2
         for (int j = 0; j < W; ++j) s = fmaf(w[j][v], win[j][v], s);
         out[v] = s;
       }
-      if (a.silu)
+      if (SILU)
 #pragma unroll
         for (int v = 0; v < V; ++v) out[v] *= nb2_sigmoid(out[v]);
       SeqVecA<T, V> o;
       o.put(out);
-      o.store(y + (tb + i) * py.stride);
+      if (i < rows) o.store(y + (tb + i) * py.stride);
     }
   }
   // The unit that read the old state writes the new one (so that the two may be the same rows): its
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_kernel(const nb2
   }
 }
 
-template <typename T, int V, int W>
+template <typename T, int V, int W, bool SILU>
 __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_grad_kernel(const nb2_causal_conv_grad_args a, int tiles) {
   nb2_pdl_enter();
   extern __shared__ __align__(16) char smem[];
@@ -246,50 +246,45 @@ __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_grad_kernel(cons
     in.get(tb, group, r);
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      const int64_t t = tb + i;
-      if (t >= t1 + W - 1) break;
-      float g[V];
+      const int64_t t = tb + i, p = t - (W - 1);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) xw[j][v] = xw[j + 1][v], gw[j][v] = gw[j + 1][v];
         xw[W - 1][v] = r[0][i][v];
-        g[v] = r[1][i][v];  // (zero past the sequence's end)
-      }
-      if (a.silu && t < len)
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
+        float g = r[1][i][v];
+        if (SILU) {
           float s = b[v];
 #pragma unroll
           for (int j = 0; j < W; ++j) s = fmaf(w[j][v], xw[j][v], s);
-          g[v] *= nb2_silu_slope(s);
+          g *= nb2_silu_slope(s);
         }
-#pragma unroll
-      for (int v = 0; v < V; ++v) gw[W - 1][v] = g[v];
+        gw[W - 1][v] = t < len ? g : 0.0f;
+      }
       if (t < t1)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          db[v] += g[v];
+          db[v] += gw[W - 1][v];
 #pragma unroll
-          for (int j = 0; j < W; ++j) dw[j][v] = fmaf(g[v], xw[j][v], dw[j][v]);
+          for (int j = 0; j < W; ++j) dw[j][v] = fmaf(gw[W - 1][v], xw[j][v], dw[j][v]);
         }
-      const int64_t p = t - (W - 1);
-      if (p < t0 && !(t0 == 0 && dstate)) continue;
-      SeqVecA<T, V> add, o;
-      add.zero();
-      if (dnew && p >= len - (W - 1)) add.load(dnew + (p - len + (W - 1)) * ns);
       float out[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        float s = add[v];
+        out[v] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < W; ++j) s = fmaf(w[W - 1 - j][v], gw[j][v], s);
-        out[v] = s;
+        for (int j = 0; j < W; ++j) out[v] = fmaf(w[W - 1 - j][v], gw[j][v], out[v]);
+      }
+      SeqVecA<T, V> o;
+      if (dnew && p >= len - (W - 1) && p < t1) {
+        o.load(dnew + (p - len + (W - 1)) * ns);
+#pragma unroll
+        for (int v = 0; v < V; ++v) out[v] += o[v];
       }
       o.put(out);
-      if (p >= 0)
+      if (p >= t0 && p < t1)
         o.store(dx + p * pdx.stride);
-      else
+      else if (t0 == 0 && p < 0 && dstate)
         o.store(dstate + (p + W - 1) * ds);
     }
   }
@@ -364,30 +359,42 @@ static cudaError_t conv_run(K kernel, dim3 grid, int smem, cudaStream_t s, const
   return nb2_launch(kernel, grid, dim3(CONV_THREADS), smem, s, a, tiles);
 }
 
-template <typename T, int V>
+template <typename T, int V, bool SILU>
 static cudaError_t conv_launch(cudaStream_t s, const nb2_causal_conv_args& a) {
   const int tiles = (a.channels + V * CONV_THREADS - 1) / (V * CONV_THREADS);
   const dim3 grid((unsigned)a.n_units * tiles);
 #define NB2_CASE(W) \
-  case W: return conv_run(nb2_causal_conv_kernel<T, V, W>, grid, ConvRows<T, V, 8, 1>::bytes() + 4 * ConvWeights<V, W>::kFloats, s, a, tiles)
+  case W: return conv_run(nb2_causal_conv_kernel<T, V, W, SILU>, grid, ConvRows<T, V, 8, 1>::bytes() + 4 * ConvWeights<V, W>::kFloats, s, a, tiles)
   switch (a.taps) {
     NB2_CASE(1); NB2_CASE(2); NB2_CASE(3); NB2_CASE(4); NB2_CASE(5); NB2_CASE(6); NB2_CASE(7);
-    default: return conv_run(nb2_causal_conv_kernel<T, V, 8>, grid, ConvRows<T, V, 8, 1>::bytes() + 4 * ConvWeights<V, 8>::kFloats, s, a, tiles);
+    default: return conv_run(nb2_causal_conv_kernel<T, V, 8, SILU>, grid, ConvRows<T, V, 8, 1>::bytes() + 4 * ConvWeights<V, 8>::kFloats, s, a, tiles);
   }
 #undef NB2_CASE
 }
 
-template <typename T, int V>
+template <typename T, int V, bool SILU>
 static cudaError_t conv_grad_launch(cudaStream_t s, const nb2_causal_conv_grad_args& a) {
   const int tiles = (a.channels + V * CONV_THREADS - 1) / (V * CONV_THREADS);
   const dim3 grid((unsigned)a.n_units * tiles);
 #define NB2_CASE(W) \
-  case W: return conv_run(nb2_causal_conv_grad_kernel<T, V, W>, grid, ConvRows<T, V, 4, 2>::bytes() + 4 * ConvWeights<V, W>::kFloats, s, a, tiles)
+  case W: return conv_run(nb2_causal_conv_grad_kernel<T, V, W, SILU>, grid, ConvRows<T, V, 4, 2>::bytes() + 4 * ConvWeights<V, W>::kFloats, s, a, tiles)
   switch (a.taps) {
     NB2_CASE(1); NB2_CASE(2); NB2_CASE(3); NB2_CASE(4); NB2_CASE(5); NB2_CASE(6); NB2_CASE(7);
-    default: return conv_run(nb2_causal_conv_grad_kernel<T, V, 8>, grid, ConvRows<T, V, 4, 2>::bytes() + 4 * ConvWeights<V, 8>::kFloats, s, a, tiles);
+    default: return conv_run(nb2_causal_conv_grad_kernel<T, V, 8, SILU>, grid, ConvRows<T, V, 4, 2>::bytes() + 4 * ConvWeights<V, 8>::kFloats, s, a, tiles);
   }
 #undef NB2_CASE
+}
+
+// Four channels to a thread whatever the type: the windows, the weights and (backward) their sums fill the registers.
+template <typename T>
+static cudaError_t conv_dispatch(cudaStream_t s, const nb2_causal_conv_args& a) {
+  if (a.vec) return a.silu ? conv_launch<T, 4, true>(s, a) : conv_launch<T, 4, false>(s, a);
+  return a.silu ? conv_launch<T, 1, true>(s, a) : conv_launch<T, 1, false>(s, a);
+}
+template <typename T>
+static cudaError_t conv_dispatch(cudaStream_t s, const nb2_causal_conv_grad_args& a) {
+  if (a.vec) return a.silu ? conv_grad_launch<T, 4, true>(s, a) : conv_grad_launch<T, 4, false>(s, a);
+  return a.silu ? conv_grad_launch<T, 1, true>(s, a) : conv_grad_launch<T, 1, false>(s, a);
 }
 
 template <typename A>
@@ -406,8 +413,7 @@ extern "C" int nb2_causal_conv(void* stream, const nb2_causal_conv_args* args) {
   const nb2_causal_conv_args& a = *args;
   if (int e = conv_check(a)) return e;
   NB2_REQUIRE(a.y, "null pointer");
-  NB2_SEQ_DTYPE(a.dtype, if (a.vec) NB2_CUDA((conv_launch<T, 16 / sizeof(T)>(nb2_stream(stream), a)));
-                else NB2_CUDA((conv_launch<T, 1>(nb2_stream(stream), a))));
+  NB2_SEQ_DTYPE(a.dtype, NB2_CUDA(conv_dispatch<T>(nb2_stream(stream), a)));
   return NB2_OK;
 }
 
@@ -416,9 +422,7 @@ extern "C" int nb2_causal_conv_grad(void* stream, const nb2_causal_conv_grad_arg
   const nb2_causal_conv_grad_args& a = *args;
   if (int e = conv_check(a)) return e;
   NB2_REQUIRE(a.dy && a.dx && a.dw && a.part, "null pointer");
-  // four channels to a thread whatever the type: the two windows, the weights and their sums are 16 W registers
-  NB2_SEQ_DTYPE(a.dtype, if (a.vec) NB2_CUDA((conv_grad_launch<T, 4>(nb2_stream(stream), a)));
-                else NB2_CUDA((conv_grad_launch<T, 1>(nb2_stream(stream), a))));
+  NB2_SEQ_DTYPE(a.dtype, NB2_CUDA(conv_dispatch<T>(nb2_stream(stream), a)));
   const int64_t n = (int64_t)(a.taps + 1) * a.channels;
   NB2_CUDA(nb2_launch(nb2_conv_grad_sum_kernel, dim3((unsigned)((n + 31) / 32)), dim3(256), 0, nb2_stream(stream), a.part,
                       a.n_units, a.taps, a.channels, a.dw, a.dbias));

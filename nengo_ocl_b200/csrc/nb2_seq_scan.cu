@@ -9,6 +9,7 @@
 // A tile of R rows is worked in three phases, each a warp's own: its lanes prepare (s, s x) of the tile's rows
 // for their channels, walk the rows through the states, and finish the outputs.
 #define SCAN_P 2
+#define SCAN_TOKEN_BLOCKS 16
 template <typename T, int S, bool VEC, bool ENDS>
 __global__ void __launch_bounds__(SCAN_THREADS, VEC ? 5 : 4) nb2_selective_scan_kernel(const nb2_selective_scan_args a) {
   constexpr int P = SCAN_P, R = NB2_SCAN_KEEP, RB = S < 4 ? S : 4;
@@ -244,72 +245,101 @@ cudaError_t nb2_scan_join(cudaStream_t s, ScanJoin j) {
   return nb2_launch(nb2_scan_join_kernel, dim3((unsigned)((j.per_seq * j.n_seq + 255) / 256)), dim3(256), 0, s, j);
 }
 
-// Single tokens and a few rows: the state is most of the traffic.  No staging; a lane loads the next
-// channel's state while it works, rows are read straight from memory.
+// Single tokens and a few rows: the states are most of the traffic, one read and one write of each.  A block keeps
+// its channels' parameters and takes one sequence after the other, the next one's state and first row on their
+// way while it works.
+constexpr int kTokenUnroll = 2;  // channels of a lane, SCAN_THREADS / S apart
+constexpr int kTokenSequences = 64, kTokenFields = 17;  // of a block; of the table: the length and eight (start, stride)
 template <typename T, int S>
-__global__ void __launch_bounds__(SCAN_THREADS) nb2_selective_scan_token_kernel(const nb2_selective_scan_args a, int tiles,
-                                                                                int per_block) {
-  constexpr int kWarp = 32 / S, kBlock = kWarp * SCAN_WARPS, kUnroll = 4;
-  nb2_pdl_enter();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = a.n_states;
-  const int k = blockIdx.x / tiles, j = lane % S, n0 = 4 * j;
-  const int per = a.channels / a.groups;
-  const int64_t len = a.table[k], nk = a.n_seq;
-  const ScanPlace px = scan_place(a.table, nk, 0, k), pt = scan_place(a.table, nk, 1, k),
-                  pb = scan_place(a.table, nk, 2, k), pc = scan_place(a.table, nk, 3, k),
-                  py = scan_place(a.table, nk, 4, k), pz = scan_place(a.table, nk, 5, k),
-                  ps = scan_place(a.table, nk, 6, k), pn = scan_place(a.table, nk, 7, k);
-  const T* x = (const T*)a.x + px.start;
-  const T* dt = (const T*)a.dt + pt.start;
-  const T* B = (const T*)a.B + pb.start;
-  const T* C = (const T*)a.C + pc.start;
-  T* y = (T*)a.y + py.start;
-  const T* z = (const T*)a.z + pz.start;
-  const int c0 = (blockIdx.x - k * tiles) * per_block, c1 = min(c0 + per_block, a.channels);
-  for (int cb = c0 + warp * kWarp + lane / S; cb - lane / S < c1; cb += kBlock * kUnroll) {
-    float h[kUnroll][4], A2[kUnroll][4], b[4], c4[4], tv[kUnroll], xv[kUnroll], zv[kUnroll], D[kUnroll], bias[kUnroll];
+struct ScanToken {
+  float h[kTokenUnroll][4], b[4], c[4], dt[kTokenUnroll], x[kTokenUnroll], z[kTokenUnroll];
+  // seq: the sequence's fields of the table
+  __device__ __forceinline__ void row(const nb2_selective_scan_args& a, const int64_t* seq, int64_t t,
+                                      const int (&ch)[kTokenUnroll], int group, int n0) {
+    const int n = a.n_states;
+    scan_load4((const T*)a.B + seq[5] + t * seq[6] + (int64_t)group * n, n0, n, a.vec, b);
+    scan_load4((const T*)a.C + seq[7] + t * seq[8] + (int64_t)group * n, n0, n, a.vec, c);
+    const T* xr = (const T*)a.x + seq[1] + t * seq[2];
+    const T* tr = (const T*)a.dt + seq[3] + t * seq[4];
+    const T* zr = a.z ? (const T*)a.z + seq[11] + t * seq[12] : nullptr;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int c = min(cb + u * kBlock, a.channels - 1);
+    for (int u = 0; u < kTokenUnroll; ++u) {
+      dt[u] = nb2_to_float(tr[ch[u]]);
+      x[u] = nb2_to_float(xr[ch[u]]);
+      z[u] = zr ? nb2_to_float(zr[ch[u]]) : 0.0f;
+    }
+  }
+  __device__ __forceinline__ void load(const nb2_selective_scan_args& a, const int64_t* seq, const int (&ch)[kTokenUnroll],
+                                       int group, int n0) {
+#pragma unroll
+    for (int u = 0; u < kTokenUnroll; ++u) {
 #pragma unroll
       for (int m = 0; m < 4; ++m) h[u][m] = 0.0f;
-      if (a.state) scan_load4(a.state + ps.start + c * ps.stride, n0, n, a.state_vec, h[u]);
-      scan_load4(a.A + (int64_t)c * n, n0, n, n % 4 == 0 && a.a_vec, A2[u]);
-      D[u] = a.D ? a.D[c] : 0.0f;
-      bias[u] = a.dt_bias ? a.dt_bias[c] : 0.0f;
+      if (a.state) scan_load4(a.state + seq[13] + ch[u] * seq[14], n0, a.n_states, a.state_vec, h[u]);
     }
-    for (int64_t t = 0; t < len; ++t) {
+    if (seq[0] > 0) row(a, seq, 0, ch, group, n0);
+  }
+};
+
+template <typename T, int S>
+__global__ void __launch_bounds__(SCAN_THREADS, 8) nb2_selective_scan_token_kernel(const nb2_selective_scan_args a, int tiles, int each) {
+  constexpr int U = kTokenUnroll, kStep = SCAN_THREADS / S;
+  __shared__ int64_t table[kTokenSequences][kTokenFields];
+  nb2_pdl_enter();
+  const int j = threadIdx.x % S, n0 = 4 * j, n = a.n_states, per = a.channels / a.groups;
+  const int tile = blockIdx.x % tiles, group = tile / (tiles / a.groups), in = (tile - group * (tiles / a.groups)) * kStep * U;
+  const int64_t k0 = (int64_t)(blockIdx.x / tiles) * each, k1 = min(k0 + each, (int64_t)a.n_seq);
+  for (int i = threadIdx.x; i < (k1 - k0) * kTokenFields; i += SCAN_THREADS)
+    table[i / kTokenFields][i % kTokenFields] = a.table[(int64_t)(i % kTokenFields) * a.n_seq + k0 + i / kTokenFields];
+  int ch[U];
+  bool valid[U];
+  float A2[U][4], D[U], bias[U];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int c = min(cb + u * kBlock, a.channels - 1);
-        tv[u] = nb2_to_float(dt[t * pt.stride + c]);
-        xv[u] = nb2_to_float(x[t * px.stride + c]);
-        zv[u] = a.z ? nb2_to_float(z[t * pz.stride + c]) : 0.0f;
-      }
+  for (int u = 0; u < U; ++u) {
+    const int at = in + u * kStep + threadIdx.x / S;
+    valid[u] = at < per;
+    ch[u] = group * per + min(at, per - 1);
+    scan_load4(a.A + (int64_t)ch[u] * n, n0, n, n % 4 == 0 && a.a_vec, A2[u]);
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int c = min(cb + u * kBlock, a.channels - 1), g = c / per;
-        scan_load4(B + t * pb.stride + g * n, n0, n, a.vec, b);
-        scan_load4(C + t * pc.stride + g * n, n0, n, a.vec, c4);
-        float s = tv[u] + bias[u], o = 0.0f;
-        if (a.softplus) s = scan_softplus(s);
-        const float sx = s * xv[u];
+    for (int m = 0; m < 4; ++m) A2[u][m] *= LOG2E;
+    D[u] = a.D ? a.D[ch[u]] : 0.0f;
+    bias[u] = a.dt_bias ? a.dt_bias[ch[u]] : 0.0f;
+  }
+  __syncthreads();
+  auto work = [&](ScanToken<T, S>& s, const int64_t* seq) {
+    for (int64_t t = 0; t < seq[0]; ++t) {
+      if (t > 0) s.row(a, seq, t, ch, group, n0);
+      T* yr = (T*)a.y + seq[9] + t * seq[10];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float step = s.dt[u] + bias[u], o = 0.0f;
+        if (a.softplus) step = scan_softplus(step);
+        const float sx = step * s.x[u];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          h[u][m] = fmaf(scan_exp2(s * (A2[u][m] * LOG2E)), h[u][m], sx * b[m]);
-          o = fmaf(c4[m], h[u][m], o);
+          s.h[u][m] = fmaf(scan_exp2(step * A2[u][m]), s.h[u][m], sx * s.b[m]);
+          o = fmaf(s.c[m], s.h[u][m], o);
         }
 #pragma unroll
         for (int w = 1; w < S; w *= 2) o += __shfl_xor_sync(0xffffffffu, o, w);
-        o = fmaf(D[u], xv[u], o);
-        if (a.z) o *= zv[u] * nb2_sigmoid(zv[u]);
-        if (j == 0 && cb + u * kBlock < c1) y[t * py.stride + c] = nb2_from_float<T>(o);
+        o = fmaf(D[u], s.x[u], o);
+        if (a.z) o *= s.z[u] * nb2_sigmoid(s.z[u]);
+        if (j == 0 && valid[u]) yr[ch[u]] = nb2_from_float<T>(o);
       }
     }
     if (a.new_state)
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (cb + u * kBlock < c1) scan_store4(a.new_state + pn.start + (cb + u * kBlock) * pn.stride, n0, n, a.state_vec, h[u]);
+      for (int u = 0; u < U; ++u)
+        if (valid[u]) scan_store4(a.new_state + seq[15] + ch[u] * seq[16], n0, n, a.state_vec, s.h[u]);
+  };
+  ScanToken<T, S> even, odd;
+  const int count = (int)(k1 - k0);
+  if (count > 0) even.load(a, table[0], ch, group, n0);
+  for (int k = 0; k < count; k += 2) {
+    if (k + 1 < count) odd.load(a, table[k + 1], ch, group, n0);
+    work(even, table[k]);
+    if (k + 2 < count) even.load(a, table[k + 2], ch, group, n0);
+    if (k + 1 < count) work(odd, table[k + 1]);
   }
 }
 
@@ -330,9 +360,11 @@ static cudaError_t scan_launch_units(cudaStream_t s, const nb2_selective_scan_ar
 template <typename T, int S>
 static cudaError_t scan_launch(cudaStream_t s, const nb2_selective_scan_args& a) {
   if (a.tokens) {
-    const int block = SCAN_THREADS / S, per_block = 4 * block, tiles = (a.channels + per_block - 1) / per_block;
-    return nb2_launch(nb2_selective_scan_token_kernel<T, S>, dim3((unsigned)a.n_seq * tiles), dim3(SCAN_THREADS), 0, s, a,
-                      tiles, per_block);
+    // as many blocks to a tile of channels as fill the GPU a few times, each with its share of the sequences
+    const int tiles = a.groups * scan_tiles(a.channels, a.groups, SCAN_THREADS / S * kTokenUnroll);
+    const int blocks = max(1, min(a.n_seq, SCAN_TOKEN_BLOCKS * NB2_NUM_SMS / tiles)), each = min((a.n_seq + blocks - 1) / blocks, kTokenSequences);
+    return nb2_launch(nb2_selective_scan_token_kernel<T, S>, dim3((unsigned)tiles * ((a.n_seq + each - 1) / each)),
+                      dim3(SCAN_THREADS), 0, s, a, tiles, each);
   }
   return a.rows_vec && a.vec ? scan_launch_units<T, S, true>(s, a) : scan_launch_units<T, S, false>(s, a);
 }

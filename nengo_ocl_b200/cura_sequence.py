@@ -32,7 +32,7 @@ MAX_TAPS = 8            # NB2_CONV_MAX_TAPS
 MAX_STATES = 128        # NB2_SCAN_MAX_STATES
 KEEP_ROWS = 16          # NB2_SCAN_KEEP
 MAX_NORM_CHANNELS = 32768  # NB2_NORM_MAX_CHANNELS
-CONV_UNITS, CONV_GRAD_UNITS = 4, 4
+CONV_UNITS, CONV_GRAD_UNITS = 8, 2
 NORM_UNITS, NORM_GRAD_UNITS = 2, 1
 TOKEN_ROWS = 4          # sequences of at most this many rows: the scan's token kernel
 
@@ -284,7 +284,7 @@ def plan_causal_conv(queue, X, W, Y, bias=None, state=None, new_state=None, acti
     width = 16 // a.dtype.itemsize
     args.vec = int(a.aligned and a.channels % width == 0)
     total = int(a.lengths.sum())
-    args.unit_rows = _unit_rows(total, -(-a.channels // (128 * (width if args.vec else 1))), 8, CONV_UNITS)
+    args.unit_rows = _unit_rows(total, -(-a.channels // (128 * (4 if args.vec else 1))), 8, CONV_UNITS)
     args.table = a.table()
     args.units, args.n_units = a.units(args.unit_rows)
     plan = _make_plan(queue, "cura_causal_conv", "nb2_causal_conv", args, a.kept, args.n_units * a.channels, 1, tag,
