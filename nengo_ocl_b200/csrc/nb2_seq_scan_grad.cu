@@ -13,6 +13,7 @@ struct ScanGradSmem {
   static constexpr int R = NB2_SCAN_KEEP;
   ScanRows<S, 1, R> ready;
   float dp[R][ScanRows<S, 1, R>::kPitch];
+  float4 sums[R][SCAN_THREADS / S];  // over the states: g B, g a h[t-1] A, C h
   alignas(16) float red[R][SCAN_WARPS][8 * S];  // dB, dC of a row: a warp's channels added
 };
 
@@ -141,7 +142,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) nb2_scan_grad_ends_kernel(const 
 }
 
 template <typename T, int S, bool VEC>
-__global__ void __launch_bounds__(SCAN_THREADS) nb2_selective_scan_grad_kernel(const nb2_selective_scan_grad_args a) {
+__global__ void __launch_bounds__(SCAN_THREADS, S < 16 && VEC ? 4 : 3) nb2_selective_scan_grad_kernel(const nb2_selective_scan_grad_args a) {
   constexpr int R = NB2_SCAN_KEEP, RB = S < 4 ? S : 4;
   constexpr int NA = 4;
   using Stage = ScanStage<T, S, 1, R, NA>;
@@ -248,89 +249,96 @@ __global__ void __launch_bounds__(SCAN_THREADS) nb2_selective_scan_grad_kernel(c
       });
     });
     __syncwarp();
-    f32x2 h[R][2], dec[R][2];
-    float out[R / RB], du[R / RB], de[R / RB];
+    // Half a tile at a time, the later one first: its decays and states stay in registers for the way back.
+    // (The later half's start costs its rows' decays once more, which the registers for 16 rows would cost in
+    // resident warps.)
+    constexpr int H = R / 2;
+    f32x2 mid[2] = {start[0], start[1]};
+    if (rows > H)
 #pragma unroll
-    for (int r0 = 0; r0 < R; r0 += RB) {
-      float p[RB];
-#pragma unroll
-      for (int i = 0; i < RB; ++i) {
-        const int r = r0 + i;
-        const float2 sx = sm.ready.sx[r][mine];
-        const f32x2 s2 = pack2(sx.x, sx.x), x2 = pack2(sx.y, sx.y);
+      for (int r = 0; r < H; ++r) {
+        f32x2 s2[1], x2[1];
+        sm.ready.get(r, mine, s2, x2);
         const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&st.bc[r][0][l.n0]);
-        const ulonglong2 cw = *reinterpret_cast<const ulonglong2*>(&st.bc[r][1][l.n0]);
-        dec[r][0] = exp2x2(mul2(s2, A2[0]));
-        dec[r][1] = exp2x2(mul2(s2, A2[1]));
-        h[r][0] = fma2(dec[r][0], r ? h[r ? r - 1 : 0][0] : start[0], mul2(x2, b.x));
-        h[r][1] = fma2(dec[r][1], r ? h[r ? r - 1 : 0][1] : start[1], mul2(x2, b.y));
-        float lo, hi;
-        unpack2(fma2(cw.y, h[r][1], mul2(cw.x, h[r][0])), lo, hi);
-        p[i] = lo + hi;
+        mid[0] = fma2(exp2x2(mul2(s2[0], A2[0])), mid[0], mul2(x2[0], b.x));
+        mid[1] = fma2(exp2x2(mul2(s2[0], A2[1])), mid[1], mul2(x2[0], b.y));
       }
-      out[r0 / RB] = 0.0f;
-      if (dz) {
-        float o = scan_transpose_sum<RB>(p, j);
+#pragma unroll 1
+    for (int rb = rows > H ? H : 0; rb >= 0; rb -= H) {
+      const f32x2 from[2] = {rb ? mid[0] : start[0], rb ? mid[1] : start[1]};
+      f32x2 h[H][2], dec[H][2];
 #pragma unroll
-        for (int w = RB; w < S; w *= 2) o += __shfl_xor_sync(0xffffffffu, o, w);
-        out[r0 / RB] = o;
+      for (int i = 0; i < H; ++i) {
+        f32x2 s2[1], x2[1];
+        sm.ready.get(rb + i, mine, s2, x2);
+        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&st.bc[rb + i][0][l.n0]);
+        dec[i][0] = exp2x2(mul2(s2[0], A2[0]));
+        dec[i][1] = exp2x2(mul2(s2[0], A2[1]));
+        h[i][0] = fma2(dec[i][0], i ? h[i ? i - 1 : 0][0] : from[0], mul2(x2[0], b.x));
+        h[i][1] = fma2(dec[i][1], i ? h[i ? i - 1 : 0][1] : from[1], mul2(x2[0], b.y));
       }
-    }
 #pragma unroll
-    for (int r0 = R - RB; r0 >= 0; r0 -= RB) {
-      float pu[RB], pe[RB];
+      for (int q = H - RB; q >= 0; q -= RB) {
+        float pu[RB], pe[RB], ps[RB];
 #pragma unroll
-      for (int i = RB - 1; i >= 0; --i) {
-        const int r = r0 + i;
-        const float2 sx = sm.ready.sx[r][mine];
-        const float dp = sm.dp[r][mine];
-        const f32x2 s2 = pack2(sx.x, sx.x), x2 = pack2(sx.y, sx.y), d2 = pack2(dp, dp);
-        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&st.bc[r][0][l.n0]);
-        const ulonglong2 cw = *reinterpret_cast<const ulonglong2*>(&st.bc[r][1][l.n0]);
-        const f32x2 g0 = fma2(cw.x, d2, carry[0]), g1 = fma2(cw.y, d2, carry[1]);
-        carry[0] = mul2(g0, dec[r][0]);
-        carry[1] = mul2(g1, dec[r][1]);
-        const f32x2 q0 = mul2(carry[0], r ? h[r ? r - 1 : 0][0] : start[0]);
-        const f32x2 q1 = mul2(carry[1], r ? h[r ? r - 1 : 0][1] : start[1]);
-        dA[0] = fma2(q0, s2, dA[0]);
-        dA[1] = fma2(q1, s2, dA[1]);
-        float lo, hi;
-        unpack2(fma2(g1, b.y, mul2(g0, b.x)), lo, hi);
-        pu[i] = lo + hi;
-        unpack2(fma2(q1, A[1], mul2(q0, A[0])), lo, hi);
-        pe[i] = lo + hi;
-        float w[8];
-        unpack2(mul2(g0, x2), w[0], w[1]);
-        unpack2(mul2(g1, x2), w[2], w[3]);
-        unpack2(mul2(d2, h[r][0]), w[4], w[5]);
-        unpack2(mul2(d2, h[r][1]), w[6], w[7]);
-        Sum::sum(w, lane);
-        if (Sum::writes(lane)) {
-          const int at = Sum::at(lane);
+        for (int i = RB - 1; i >= 0; --i) {
+          const int r = rb + q + i;
+          f32x2 s2[1], x2[1];
+          sm.ready.get(r, mine, s2, x2);
+          const float dp = sm.dp[r][mine];
+          const f32x2 d2 = pack2(dp, dp);
+          const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&st.bc[r][0][l.n0]);
+          const ulonglong2 cw = *reinterpret_cast<const ulonglong2*>(&st.bc[r][1][l.n0]);
+          const f32x2 h0 = h[q + i][0], h1 = h[q + i][1];
+          const f32x2 g0 = fma2(cw.x, d2, carry[0]), g1 = fma2(cw.y, d2, carry[1]);
+          carry[0] = mul2(g0, dec[q + i][0]);
+          carry[1] = mul2(g1, dec[q + i][1]);
+          const f32x2 q0 = mul2(carry[0], q + i ? h[q + i ? q + i - 1 : 0][0] : from[0]);
+          const f32x2 q1 = mul2(carry[1], q + i ? h[q + i ? q + i - 1 : 0][1] : from[1]);
+          dA[0] = fma2(q0, s2[0], dA[0]);
+          dA[1] = fma2(q1, s2[0], dA[1]);
+          float lo, hi;
+          unpack2(fma2(g1, b.y, mul2(g0, b.x)), lo, hi);
+          pu[i] = lo + hi;
+          unpack2(fma2(q1, A[1], mul2(q0, A[0])), lo, hi);
+          pe[i] = lo + hi;
+          unpack2(fma2(cw.y, h1, mul2(cw.x, h0)), lo, hi);
+          ps[i] = lo + hi;
+          float w[8];
+          unpack2(mul2(g0, x2[0]), w[0], w[1]);
+          unpack2(mul2(g1, x2[0]), w[2], w[3]);
+          unpack2(mul2(d2, h0), w[4], w[5]);
+          unpack2(mul2(d2, h1), w[6], w[7]);
+          Sum::sum(w, lane);
+          if (Sum::writes(lane)) {
+            const int at = Sum::at(lane);
 #pragma unroll
-          for (int m = 0; m < Sum::kLeft; ++m) sm.red[r][warp][((at + m) >> 2) * 4 * S + l.n0 + ((at + m) & 3)] = w[m];
+            for (int m = 0; m < Sum::kLeft; ++m) sm.red[r][warp][((at + m) >> 2) * 4 * S + l.n0 + ((at + m) & 3)] = w[m];
+          }
         }
-      }
-      float u = scan_transpose_sum<RB>(pu, j), e = scan_transpose_sum<RB>(pe, j);
+        float u = scan_transpose_sum<RB>(pu, j), e = scan_transpose_sum<RB>(pe, j), o = scan_transpose_sum<RB>(ps, j);
 #pragma unroll
-      for (int w = RB; w < S; w *= 2) {
-        u += __shfl_xor_sync(0xffffffffu, u, w);
-        e += __shfl_xor_sync(0xffffffffu, e, w);
+        for (int w = RB; w < S; w *= 2) {
+          u += __shfl_xor_sync(0xffffffffu, u, w);
+          e += __shfl_xor_sync(0xffffffffu, e, w);
+          o += __shfl_xor_sync(0xffffffffu, o, w);
+        }
+        if (RB == S || l.j < RB) sm.sums[rb + q + j][mine] = make_float4(u, e, o, 0.0f);
       }
-      du[r0 / RB] = u;
-      de[r0 / RB] = e;
     }
+    __syncwarp();
     scan_switch(a.softplus, [&](auto soft) {
       scan_switch(dz != nullptr, [&](auto gated) {
 #pragma unroll
         for (int r0 = 0; r0 < R; r0 += RB) {
           const int r = r0 + j;
           const float raw = nb2_to_float(st.in[0][r][mine]) + bias, xv = nb2_to_float(st.in[1][r][mine]);
-          const float dp = sm.dp[r][mine], u = du[r0 / RB];
-          float ds = fmaf(xv, u, de[r0 / RB]), gz = 0.0f;
+          const float4 sum = sm.sums[r][mine];
+          const float dp = sm.dp[r][mine], u = sum.x;
+          float ds = fmaf(xv, u, sum.y), gz = 0.0f;
           if (decltype(soft)::value) ds *= nb2_sigmoid(raw);
           if (decltype(gated)::value)
-            gz = nb2_to_float(st.in[2][r][mine]) * fmaf(D, xv, out[r0 / RB]) * nb2_silu_slope(nb2_to_float(st.in[3][r][mine]));
+            gz = nb2_to_float(st.in[2][r][mine]) * fmaf(D, xv, sum.z) * nb2_silu_slope(nb2_to_float(st.in[3][r][mine]));
           if (r < rows && stores) {
             dx[(tb + r) * pdx.stride] = nb2_from_float<T>(fmaf(D, dp, sm.ready.sx[r][mine].x * u));
             ddt[(tb + r) * pdt.stride] = nb2_from_float<T>(ds);
