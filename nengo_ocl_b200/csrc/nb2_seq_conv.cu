@@ -307,6 +307,7 @@ __global__ void __launch_bounds__(256) nb2_conv_grad_sum_kernel(const float* par
   const int64_t n = (int64_t)(taps + 1) * channels, i = (int64_t)blockIdx.x * 32 + lane;
   float s = 0.0f;
   if (i < n)
+#pragma unroll 8
     for (int u = w; u < n_units; u += 8) s += part[(int64_t)u * n + i];
   run[w][lane] = s;
   __syncthreads();
@@ -331,6 +332,7 @@ __global__ void __launch_bounds__(256) nb2_seq_sum_parts_kernel(const float* par
     const int64_t i = b * 32 + lane;
     float s = 0.0f;
     if (i < n)
+#pragma unroll 8
       for (int64_t u = w; u < n_parts; u += 8) s += part[u * n + i];
     run[w][lane] = s;
     __syncthreads();

@@ -222,6 +222,7 @@ __global__ void __launch_bounds__(256) nb2_norm_grad_sum_kernel(const nb2_residu
   const int64_t n = 2ll * a.channels, i = (int64_t)blockIdx.x * 32 + lane;
   float s = 0.0f;
   if (i < n)
+#pragma unroll 8
     for (int u = w; u < a.n_units; u += 8) s += a.part[(int64_t)u * n + i];
   run[w][lane] = s;
   __syncthreads();

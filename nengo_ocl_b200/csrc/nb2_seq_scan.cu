@@ -72,7 +72,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, VEC ? 5 : 4) nb2_selective_scan_
   auto arrive = [&](Stage& st) {
     weights.store(st.bc, n);
 #pragma unroll
-    for (int i = 0; i < NA; ++i) copy[i].store(st.in[i]);
+    for (int i = 0; i < NA; ++i)
+      if (i < 2 || z) copy[i].store(st.in[i]);
   };
   const int64_t all = t1 - t0;
   if (all > 0) {

@@ -397,6 +397,7 @@ __global__ void __launch_bounds__(256) nb2_scan_grad_bc_kernel(const nb2_selecti
     const int64_t r = i / wide;
     const int rest = (int)(i - r * wide), group = rest / (2 * n), m = rest - group * 2 * n;
     float sum = 0.0f;
+#pragma unroll 8
     for (int u = 0; u < tiles; ++u) sum += a.part_bc[u * all + (row0 + r) * wide + rest];
     if (m < n)
       ((T*)a.dB)[pb.start + r * pb.stride + group * n + m] = nb2_from_float<T>(sum);

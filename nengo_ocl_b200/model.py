@@ -332,6 +332,48 @@ class SimVoja(Operator):
         self.updates = [delta]
 
 
+class SimCausalConv(Operator):
+    """One step of a short causal convolution, channel by channel (``plan_causal_conv`` on single tokens):
+    ``y = act(bias + sum_j weights[:, j] * x[taps - 1 - j steps ago])``; ``state`` (taps - 1, channels) holds the
+    last inputs, oldest first.  ``weights``: (channels, taps), taps >= 2."""
+
+    def __init__(self, x, weights, y, state, bias=None, activation=None, tag=None):
+        super().__init__(tag)
+        self.x, self.weights, self.y, self.state, self.bias = x, weights, y, state, bias
+        self.activation = activation
+        self.sets = [y]
+        self.reads = [s for s in (x, weights, bias) if s is not None]
+        self.updates = [state]
+
+
+class SimSelectiveScan(Operator):
+    """One step of a selective state space scan (``plan_selective_scan`` on single tokens): the linear filter
+    whose step size ``dt`` and weights ``B``, ``C`` are signals.  ``A``, ``state``: (channels, n_states);
+    ``B``, ``C``: (groups * n_states,); ``D``, ``dt_bias``, ``z``: (channels,) or None."""
+
+    def __init__(self, x, dt, A, B, C, y, state, D=None, z=None, dt_bias=None, softplus=True, tag=None):
+        super().__init__(tag)
+        self.x, self.dt, self.A, self.B, self.C, self.y, self.state = x, dt, A, B, C, y, state
+        self.D, self.z, self.dt_bias, self.softplus = D, z, dt_bias, bool(softplus)
+        self.sets = [y]
+        self.reads = [s for s in (x, dt, A, B, C, D, z, dt_bias) if s is not None]
+        self.updates = [state]
+
+
+class SimResidualNorm(Operator):
+    """Gate, norm, residual and the next norm of one step (``plan_residual_norm`` on single tokens); ``scale``:
+    a number or a (channels,) signal, ``y`` or ``h`` may be None."""
+
+    def __init__(self, x, y=None, h=None, gate=None, gate_first=True, residual=None, weight=None, scale=1.0,
+                 norm_weight=None, groups=1, eps=1e-5, tag=None):
+        super().__init__(tag)
+        self.x, self.y, self.h, self.gate, self.gate_first = x, y, h, gate, bool(gate_first)
+        self.residual, self.weight, self.scale, self.norm_weight = residual, weight, scale, norm_weight
+        self.groups, self.eps = int(groups), float(eps)
+        self.sets = [s for s in (y, h) if s is not None]
+        self.reads = [s for s in (x, gate, residual, weight, norm_weight, scale) if isinstance(s, Signal)]
+
+
 class SimPyFunc(Operator):
     def __init__(self, output, fn, t, x, tag=None):
         super().__init__(tag)

@@ -47,6 +47,7 @@ from nengo_ocl_b200.cura_nonlinearities import (
     plan_voja,
 )
 from nengo_ocl_b200.curaggedarray import CUDARaggedArray, to_device
+from nengo_ocl_b200.model import Signal
 from nengo_ocl_b200.operators import MultiDotInc, simplify_operators
 from nengo_ocl_b200.plan import BasePlan, Plans, PythonPlan
 from nengo_ocl_b200.planners import greedy_planner
@@ -1072,6 +1073,61 @@ class Simulator:
                                                          "delta", "learning_signal")
         scale = self.RaggedArray([np.asarray(op.scale).reshape(-1, 1) for op in ops], dtype=np.float32)
         return [plan_voja(self.queue, pre, post, encoders, delta, learn, scale, self._scaled_rates(ops))]
+
+    # ---- sequence operators, one row (token) a step --------------------------------
+    def _row_items(self, signals):
+        """Device view of vector signals as rows of one token each."""
+        if signals[0] is None:
+            return None
+        items = self._items(signals)
+        n = items.shape0s
+        return CUDARaggedArray.from_buffer(self.queue, items.cl_buf, items.starts, np.ones_like(n), n, n, items.stride0s)
+
+    def _parameter(self, signal):
+        return None if signal is None else self.all_data.getitem_device(self.sidx[signal])
+
+    def _plan_sequence_ops(self, ops, shared, same, rows, make):
+        plans = []
+        key = lambda op: (tuple(getattr(op, n) if not isinstance(getattr(op, n), Signal) else id(getattr(op, n))
+                                for n in shared + same), op.x.size, tuple(getattr(op, n) is None for n in rows))
+        for _, group in groupby(ops, key):
+            args = {n: self._row_items([getattr(op, n) for op in group]) for n in rows}
+            args.update({n: self._parameter(getattr(group[0], n)) if isinstance(getattr(group[0], n), (Signal, type(None)))
+                         else getattr(group[0], n) for n in shared})
+            args.update({n: getattr(group[0], n) for n in same})
+            plans.append(make(group, args))
+        return plans
+
+    def _plan_SimCausalConv(self, ops):
+        from nengo_ocl_b200.cura_sequence import plan_causal_conv
+
+        def make(group, a):
+            state = self._items([op.state for op in group])
+            return plan_causal_conv(self.queue, a["x"], a["weights"], a["y"], bias=a["bias"], state=state,
+                                    new_state=state, activation=a["activation"])
+
+        return self._plan_sequence_ops(ops, ("weights", "bias"), ("activation",), ("x", "y"), make)
+
+    def _plan_SimSelectiveScan(self, ops):
+        from nengo_ocl_b200.cura_sequence import plan_selective_scan
+
+        def make(group, a):
+            state = self._items([op.state for op in group])
+            return plan_selective_scan(self.queue, a["x"], a["dt"], a["A"], a["B"], a["C"], a["y"], D=a["D"], Z=a["z"],
+                                       dt_bias=a["dt_bias"], softplus=a["softplus"], state=state, new_state=state)
+
+        return self._plan_sequence_ops(ops, ("A", "D", "dt_bias"), ("softplus",), ("x", "dt", "B", "C", "y", "z"), make)
+
+    def _plan_SimResidualNorm(self, ops):
+        from nengo_ocl_b200.cura_sequence import plan_residual_norm
+
+        def make(group, a):
+            return plan_residual_norm(self.queue, a["x"], Y=a["y"], H=a["h"], gate=a["gate"], gate_first=a["gate_first"],
+                                      residual=a["residual"], weight=a["weight"], scale=a["scale"],
+                                      norm_weight=a["norm_weight"], groups=a["groups"], eps=a["eps"])
+
+        return self._plan_sequence_ops(ops, ("weight", "scale", "norm_weight"), ("gate_first", "groups", "eps"),
+                                       ("x", "y", "h", "gate", "residual"), make)
 
     def _plan_SimRLS(self, ops):
         raise NotImplementedError("RLS learning rule not yet supported")  # (nor in the reference, :1372)

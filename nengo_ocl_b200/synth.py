@@ -570,3 +570,37 @@ def convolution_model(seed=31, channels_last=True, one_d=False):
     probes = [mdl.add_probe(y2, label="y2"), mdl.add_probe(j1, label="j1")]
     mdl.info = dict(probes=probes, signals=[image, j1, r1, y2], convs=(conv1, conv2))
     return mdl
+
+
+def state_space_model(seed=41, n_streams=2, channels=48, n_states=16, taps=4):
+    """Streams of noise through one block of a state space network, stepped once per time step: norm, short
+    causal convolution, projections of its output to the scan's step size and weights, selective scan, and the
+    gated norm that adds its result to the stream.  The streams share the parameters."""
+    rng = np.random.RandomState(seed)
+    mdl = m.Model(dt=0.001)
+    const = lambda name, v: m.Signal(np.asarray(v, dtype=np.float64), name=name, readonly=True)
+    norm_w, post_w, scale = (const(n, rng.uniform(0.5, 1.5, size=channels)) for n in ("norm_w", "post_w", "scale"))
+    conv_w, conv_b = const("conv_w", rng.normal(scale=0.5, size=(channels, taps))), const("conv_b", rng.normal(size=channels))
+    A = const("A", -rng.uniform(0.5, n_states, size=(channels, n_states)))
+    D, dt_bias = const("D", rng.normal(size=channels)), const("dt_bias", rng.uniform(-5, -2, size=channels))
+    project = {n: const("W_" + n, rng.normal(scale=channels ** -0.5, size=(size, channels)))
+               for n, size in (("dt", channels), ("B", n_states), ("C", n_states), ("z", channels))}
+    probes, states = [], []
+    for k in range(n_streams):
+        sig = lambda name, *shape: m.Signal(np.zeros(shape or channels), name="%s%d" % (name, k))
+        stream, normed, conv, scanned, out = (sig(n) for n in ("stream", "normed", "conv", "scanned", "out"))
+        dt, B, C, z = sig("dt"), sig("B", n_states), sig("C", n_states), sig("z")
+        conv_state, state = sig("conv_state", taps - 1, channels), sig("state", channels, n_states)
+        noise = m.WhiteNoise(m.Uniform(-1, 1), scale=False, seed=seed + k)
+        mdl.add_op(m.SimProcess(noise, None, stream, mdl.step, mode="set"))
+        mdl.add_op(m.SimResidualNorm(stream, h=normed, norm_weight=norm_w))
+        mdl.add_op(m.SimCausalConv(normed, conv_w, conv, conv_state, bias=conv_b, activation="silu"))
+        for name, source, target in (("dt", conv, dt), ("B", conv, B), ("C", conv, C), ("z", normed, z)):
+            mdl.add_op(m.Reset(target))
+            mdl.add_op(m.DotInc(project[name], source, target))
+        mdl.add_op(m.SimSelectiveScan(conv, dt, A, B, C, scanned, state, D=D, dt_bias=dt_bias))
+        mdl.add_op(m.SimResidualNorm(scanned, y=out, gate=z, residual=stream, weight=post_w, scale=scale))
+        probes.append(mdl.add_probe(out, label="out%d" % k))
+        states.append((conv_state, state))
+    mdl.info = dict(probes=probes, states=states)
+    return mdl

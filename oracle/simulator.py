@@ -334,6 +334,39 @@ class OracleSimulator:
         alpha = f32(-op.learning_rate * self.dt / pre.shape[0])
         delta[...] = ((alpha * err)[:, None] * pre[None, :]).astype(np.float32)
 
+    # sequence operators, one row a step: the float64 formulas, rounded once
+    def _row(self, sig):
+        return None if sig is None else self.view(sig).reshape(1, -1)
+
+    def _vector(self, sig):
+        return self.view(sig).reshape(-1) if hasattr(sig, "base") else sig
+
+    def _do_SimCausalConv(self, op):
+        from oracle import sequences as S
+
+        y, state = S.causal_conv(self._row(op.x), self.view(op.weights), self._vector(op.bias), self.view(op.state),
+                                 op.activation == "silu")
+        self.view(op.y).reshape(-1)[...] = y[0]
+        self.view(op.state)[...] = state
+
+    def _do_SimSelectiveScan(self, op):
+        from oracle import sequences as S
+
+        y, state = S.selective_scan(self._row(op.x), self._row(op.dt), self.view(op.A), self._row(op.B), self._row(op.C),
+                                    self._vector(op.D), self._row(op.z), self._vector(op.dt_bias), op.softplus,
+                                    self.view(op.state))
+        self.view(op.y).reshape(-1)[...] = y[0]
+        self.view(op.state)[...] = state
+
+    def _do_SimResidualNorm(self, op):
+        from oracle import sequences as S
+
+        y, h = S.residual_norm(self._row(op.x), self._row(op.gate), op.gate_first, self._row(op.residual),
+                               self._vector(op.weight), self._vector(op.scale), self._vector(op.norm_weight), op.groups, op.eps)
+        for sig, value in ((op.y, y), (op.h, h)):
+            if sig is not None:
+                self.view(sig).reshape(-1)[...] = value[0]
+
     def _do_SimBCM(self, op):
         self.view(op.delta)[...] = K.bcm(self.view(op.pre_filtered), self.view(op.post_filtered),
                                          self.view(op.theta), op.learning_rate * self.dt)

@@ -370,3 +370,48 @@ def test_queue_over_an_existing_stream(fake_queue):
     assert q.stream == 0
     x = to_device(q, np.arange(4, dtype=np.float32))
     assert np.array_equal(x.get(), np.arange(4))
+
+
+# ---- in a simulated model ------------------------------------------------------------------------
+def test_model_operators_are_planned_once_per_parameter_set(monkeypatch):
+    from nengo_ocl_b200 import runtime, synth
+    from nengo_ocl_b200 import simulator as sim_mod
+
+    fake_library.install(monkeypatch)
+    monkeypatch.setattr(sim_mod.Simulator, "some_context", None)
+    monkeypatch.setattr(runtime, "_default_context", None, raising=False)
+    sim = sim_mod.Simulator(None, model=synth.state_space_model(n_streams=3))
+    names = [p.name for p in sim._plans]
+    assert names.count("cura_causal_conv") == names.count("cura_selective_scan") == 1
+    assert names.count("cura_residual_norm") == 2  # before and after the block
+    ours = ("cura_residual_norm", "cura_causal_conv", "cura_selective_scan")
+    order = [n for n in names if n in ours]
+    assert order == ["cura_residual_norm", "cura_causal_conv", "cura_selective_scan", "cura_residual_norm"]
+    for p in sim._plans:
+        if p.name in ours:
+            assert len(p.sequence_args["X"]) == 3 and (p.sequence_args["X"].shape0s == 1).all()
+            assert p.signal_use is not None
+    sim.close()
+
+
+def test_oracle_steps_equal_whole_sequences():
+    """The operator-list interpreter's step-by-step block against one pass over all rows."""
+    from nengo_ocl_b200 import synth
+    from oracle.simulator import OracleSimulator
+
+    mdl = synth.state_space_model(n_streams=1)
+    ora = OracleSimulator(mdl)
+    conv_state, state = mdl.info["states"][0]
+    by_name = {s.name: s for op in mdl.operators for s in op.all_signals}
+    rows = {n: [] for n in ("normed0", "conv0", "dt0", "B0", "C0", "scanned0")}
+    for _ in range(12):
+        ora.step()
+        for n, v in rows.items():
+            v.append(ora[by_name[n]].reshape(-1))
+    rows = {n: np.array(v) for n, v in rows.items()}
+    get = lambda n: ora[by_name[n]].astype(float)
+    y, end = S.causal_conv(rows["normed0"], get("conv_w"), get("conv_b"), None, True)
+    assert np.allclose(y, rows["conv0"], rtol=1e-6, atol=1e-6) and np.array_equal(end, ora[conv_state])
+    y, end = S.selective_scan(rows["conv0"], rows["dt0"], get("A"), rows["B0"], rows["C0"], get("D"), None, get("dt_bias"), True)
+    # (the state is rounded to float32 after every step: 12 half steps)
+    assert np.allclose(y, rows["scanned0"], rtol=1e-5, atol=1e-5) and np.allclose(end, ora[state], rtol=1e-5, atol=1e-6)

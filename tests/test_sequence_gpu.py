@@ -610,3 +610,29 @@ def test_the_plans_device_must_be_current(queue, rng):
     plan()
     s.check()
     assert ctypes.sizeof(args) > 0
+
+
+# ---- in a simulated model ------------------------------------------------------------------------
+def test_simulated_block_matches_the_oracle(ctx):
+    from nengo_ocl_b200 import synth
+    from nengo_ocl_b200.simulator import Simulator
+    from oracle.simulator import OracleSimulator
+
+    mdl = synth.state_space_model()
+    ora = OracleSimulator(mdl)
+    ora.run_steps(40)
+    with Simulator(None, model=mdl, context=ctx) as sim:
+        first = None
+        for _ in range(2):  # again after a reset: the states start over
+            sim.run_steps(40)
+            for p in mdl.info["probes"]:
+                want = np.array(ora.probe_data[p])
+                # values of order one; float32 products over 48 channels and 40 rows of a decaying state
+                assert np.allclose(sim.data[p], want, rtol=1e-4, atol=1e-4)
+            for pair in mdl.info["states"]:
+                for s in pair:
+                    assert np.allclose(sim.signals[s], ora[s], rtol=1e-4, atol=1e-4)
+            data = [np.array(sim.data[p]) for p in mdl.info["probes"]]
+            assert first is None or all(np.array_equal(a, b) for a, b in zip(first, data))
+            first = data
+            sim.reset()
