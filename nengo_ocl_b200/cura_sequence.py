@@ -24,7 +24,7 @@ import numpy as np
 from nengo_ocl_b200 import _capi
 from nengo_ocl_b200.curaggedarray import CUDARaggedArray
 from nengo_ocl_b200.plan import Plan
-from nengo_ocl_b200.runtime import DeviceArray, to_device
+from nengo_ocl_b200.runtime import DeviceArray
 from nengo_ocl_b200.utils import bfloat16, is_number
 
 _DTYPES = {np.dtype(np.float32): 0, np.dtype(np.float16): 1, bfloat16: 2}
@@ -109,6 +109,7 @@ class _Arguments:
         self.memory = []
         self.fields = []
         self.kept = []
+        self.blocks = []
         self.aligned = True
 
     def rows(self, name, ra, columns=None, lengths=None, dtype=None, written=False, optional=False, vec=True):
@@ -207,25 +208,48 @@ class _Arguments:
                             continue
                     raise ValueError("%s, which is written, overlaps %s" % (m.name, o.name))
 
+    # A plan's tables and scratch are one allocation and one upload: `table`, `units` and `scratch` note what is
+    # needed and return a token, `place` puts the addresses into the launch's arguments.
+    def _need(self, nbytes, host=None):
+        self.blocks.append((int(nbytes), host))
+        return len(self.blocks) - 1
+
     def table(self, *more):
-        out = to_device(self.queue, np.stack([self.lengths] + self.fields + list(more)).astype(np.int64))
-        self.kept.append(out)
-        return out.data
+        host = np.ascontiguousarray(np.stack([self.lengths] + self.fields + list(more)).astype(np.int64))
+        return self._need(host.nbytes, host)
 
     def units(self, rows):
         """(sequence, first row) of every stretch of ``rows`` rows; one for an empty sequence too."""
         n = np.maximum(-(-self.lengths // rows), 1)
         seq = np.repeat(np.arange(len(n)), n)
         first = (np.arange(len(seq)) - np.repeat(np.cumsum(n) - n, n)) * rows
-        if len(first) and first.max() >= 2 ** 31:
+        if first.max() >= 2 ** 31:
             raise NotImplementedError("sequences of 2^31 rows")
-        self.kept.append(to_device(self.queue, np.stack([seq, first], axis=1).astype(np.int32)))
-        return self.kept[-1].data, len(seq)
+        host = np.ascontiguousarray(np.stack([seq, first], axis=1).astype(np.int32))
+        return self._need(host.nbytes, host), len(seq)
 
     def scratch(self, n):
-        out = DeviceArray(self.queue, (max(int(n), 1),), np.float32)
-        self.kept.append(out)
-        return out.data
+        return self._need(4 * max(int(n), 1))
+
+    def place(self, args, **tokens):
+        """Allocates what was asked for and sets the fields ``name=token`` of ``args``."""
+        up = lambda n: (n + 255) // 256 * 256
+        order = sorted(range(len(self.blocks)), key=lambda i: self.blocks[i][1] is None)  # what is uploaded first
+        offsets, total, upload = {}, 0, 0
+        for i in order:
+            offsets[i] = total
+            total += up(self.blocks[i][0])
+            upload = total if self.blocks[i][1] is not None else upload
+        memory = DeviceArray(self.queue, (total,), np.uint8)
+        host = np.zeros(upload, np.uint8)
+        for i, (nbytes, data) in enumerate(self.blocks):
+            if data is not None:
+                host[offsets[i]:offsets[i] + nbytes] = data.view(np.uint8).reshape(-1)
+        memory.write_region(0, host)
+        self.kept.append(memory)
+        for name, token in tokens.items():
+            if token is not None:
+                setattr(args, name, memory.data + offsets[token])
 
     def common(self):
         return dict(device=self.queue.context.ordinal, dtype=_DTYPES[self.dtype], n_seq=len(self.lengths),
@@ -285,8 +309,8 @@ def plan_causal_conv(queue, X, W, Y, bias=None, state=None, new_state=None, acti
     args.vec = int(a.aligned and a.channels % width == 0)
     total = int(a.lengths.sum())
     args.unit_rows = _unit_rows(total, -(-a.channels // (128 * (4 if args.vec else 1))), 8, CONV_UNITS)
-    args.table = a.table()
-    args.units, args.n_units = a.units(args.unit_rows)
+    units, args.n_units = a.units(args.unit_rows)
+    a.place(args, table=a.table(), units=units)
     plan = _make_plan(queue, "cura_causal_conv", "nb2_causal_conv", args, a.kept, args.n_units * a.channels, 1, tag,
                       total * a.channels * (2 * taps + 4), _nbytes(a.memory))
     plan.sequence_args = dict(X=X, W=W, bias=bias, state=state, new_state=new_state, activation=activation)
@@ -327,9 +351,8 @@ def plan_causal_conv_grad(queue, plan, dY, dX, dW, dbias=None, dstate=None, dnew
     args.vec = int(a.aligned and a.channels % width == 0)
     total = int(a.lengths.sum())
     args.unit_rows = _unit_rows(total, -(-a.channels // (128 * (4 if args.vec else 1))), 16, CONV_GRAD_UNITS)
-    args.table = a.table()
-    args.units, args.n_units = a.units(args.unit_rows)
-    args.part = a.scratch(args.n_units * (taps + 1) * a.channels)
+    units, args.n_units = a.units(args.unit_rows)
+    a.place(args, table=a.table(), units=units, part=a.scratch(args.n_units * (taps + 1) * a.channels))
     return _make_plan(queue, "cura_causal_conv_grad", "nb2_causal_conv_grad", args, a.kept,
                       args.n_units * a.channels, 2, tag, total * a.channels * (6 * taps + 10), moved)
 
@@ -347,17 +370,18 @@ def scan_tile(n_states, backward=False):
 def _scan_units(a, args, tiles, want):
     """Splits the sequences into units of rows.  A block walks a unit row after row, so a batch of few channels
     or one long sequence is split over time until there are ``want`` blocks; that computes every row's
-    decay twice (once for the units' ends).  Returns the sequences' first units."""
+    decay twice (once for the units' ends).  Returns the sequences' first units and what to place."""
     longest, total = max(int(a.lengths.max()), 1), int(a.lengths.sum())
     args.unit_rows = -(-longest // 32) * 32
     if len(a.lengths) * tiles < want // 2 and longest > 128:
         args.unit_rows = min(args.unit_rows, max(64, -(-total * tiles // (want * 32)) * 32))
     units = np.maximum(-(-a.lengths // args.unit_rows), 1)
-    args.units, args.n_units = a.units(args.unit_rows)
+    tokens = dict.fromkeys(("units", "ends", "sums"))
+    tokens["units"], args.n_units = a.units(args.unit_rows)
     if args.n_units > len(a.lengths):
-        args.ends = a.scratch(args.n_units * a.channels * args.n_states)
-        args.sums = a.scratch(args.n_units * a.channels)
-    return np.cumsum(units) - units
+        tokens["ends"] = a.scratch(args.n_units * a.channels * args.n_states)
+        tokens["sums"] = a.scratch(args.n_units * a.channels)
+    return np.cumsum(units) - units, tokens
 
 
 def plan_selective_scan(queue, X, dt, A, B, C, Y, D=None, Z=None, dt_bias=None, softplus=False, state=None,
@@ -408,15 +432,14 @@ def plan_selective_scan(queue, X, dt, A, B, C, Y, D=None, Z=None, dt_bias=None, 
     moved = _nbytes(a.memory)
     blocks = -(-a.lengths // KEEP_ROWS)
     first = np.cumsum(blocks) - blocks
-    if keep:
-        args.keep = a.scratch(int(blocks.sum()) * a.channels * n)
+    kept = a.scratch(int(blocks.sum()) * a.channels * n) if keep else None
     longest = int(a.lengths.max())
     args.tokens = int(longest <= TOKEN_ROWS and not keep)
-    launches, first_unit = 1, np.arange(len(a.lengths))
+    launches, first_unit, tokens = 1, np.arange(len(a.lengths)), {}
     if not args.tokens:
-        first_unit = _scan_units(a, args, groups * -(-(a.channels // groups) // scan_tile(n)), 148 * 8)
-        launches = 3 if args.ends else 1
-    args.table = a.table(first, first_unit)
+        first_unit, tokens = _scan_units(a, args, groups * -(-(a.channels // groups) // scan_tile(n)), 148 * 8)
+        launches = 3 if tokens["ends"] is not None else 1
+    a.place(args, table=a.table(first, first_unit), keep=kept, **tokens)
     total = int(a.lengths.sum())
     plan = _make_plan(queue, "cura_selective_scan", "nb2_selective_scan", args, a.kept, len(a.lengths) * a.channels,
                       launches, tag, total * a.channels * (7 * n + 20), moved)
@@ -471,12 +494,10 @@ def plan_selective_scan_grad(queue, plan, dY, dX, ddt, dA, dB, dC, dD=None, dZ=N
     total = int(a.lengths.sum())
     args.total_rows = total
     tiles = -(-(a.channels // groups) // scan_tile(n, backward=True))
-    first_unit = _scan_units(a, args, groups * tiles, 148 * 8)
-    args.table = a.table(f["first"], np.cumsum(a.lengths) - a.lengths, first_unit, np.zeros_like(first_unit))
-    args.part_bc = a.scratch(tiles * total * 2 * width)
-    args.part_a = a.scratch(args.n_units * a.channels * n)
-    args.part_d = a.scratch(args.n_units * a.channels)
-    args.part_s = a.scratch(args.n_units * a.channels)
+    first_unit, tokens = _scan_units(a, args, groups * tiles, 148 * 8)
+    a.place(args, table=a.table(f["first"], np.cumsum(a.lengths) - a.lengths, first_unit, np.zeros_like(first_unit)),
+            part_bc=a.scratch(tiles * total * 2 * width), part_a=a.scratch(args.n_units * a.channels * n),
+            part_d=a.scratch(args.n_units * a.channels), part_s=a.scratch(args.n_units * a.channels), **tokens)
     return _make_plan(queue, "cura_selective_scan_grad", "nb2_selective_scan_grad", args, a.kept,
                       len(a.lengths) * a.channels, 5 + 2 * bool(args.ends), tag, total * a.channels * (19 * n + 30), moved)
 
@@ -524,8 +545,8 @@ def plan_residual_norm(queue, X, Y=None, H=None, gate=None, gate_first=True, res
     args.param_vec = int(not any(p % 16 for p in (args.weight, args.scale, args.norm_weight) if p))
     total = int(a.lengths.sum())
     args.unit_rows = max(1, -(-total // (148 * NORM_UNITS)))
-    args.table = a.table()
-    args.units, args.n_units = a.units(args.unit_rows)
+    units, args.n_units = a.units(args.unit_rows)
+    a.place(args, table=a.table(), units=units)
     plan = _make_plan(queue, "cura_residual_norm", "nb2_residual_norm", args, a.kept, total * a.channels, 1, tag,
                       total * a.channels * 16, moved)
     plan.sequence_args = dict(X=X, gate=gate, gate_first=gate_first, residual=residual, weight=weight, scale=scale,
@@ -570,8 +591,7 @@ def plan_residual_norm_grad(queue, plan, dX, dY=None, dH=None, dgate=None, dresi
     args.param_vec = int(not any(p % 16 for p in (args.weight, args.scale, args.norm_weight) if p))
     total = int(a.lengths.sum())
     args.unit_rows = max(1, -(-total // (148 * NORM_GRAD_UNITS)))
-    args.table = a.table()
-    args.units, args.n_units = a.units(args.unit_rows)
-    args.part = a.scratch(args.n_units * 2 * a.channels)
+    units, args.n_units = a.units(args.unit_rows)
+    a.place(args, table=a.table(), units=units, part=a.scratch(args.n_units * 2 * a.channels))
     return _make_plan(queue, "cura_residual_norm_grad", "nb2_residual_norm_grad", args, a.kept, total * a.channels,
                       2, tag, total * a.channels * 40, moved)
