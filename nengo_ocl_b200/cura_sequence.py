@@ -32,9 +32,21 @@ MAX_TAPS = 8            # NB2_CONV_MAX_TAPS
 MAX_STATES = 128        # NB2_SCAN_MAX_STATES
 KEEP_ROWS = 16          # NB2_SCAN_KEEP
 MAX_NORM_CHANNELS = 32768  # NB2_NORM_MAX_CHANNELS
+
+# Launch shapes, chosen by measurement on a B200 (148 multiprocessors).
+# Units a multiprocessor of the convolution (rows of a unit are halved, 64 to 8, until there are so many): 2 / 4 / 8 / 16
+# units 44.6 / 44.9 / 41.5 / 45.0 us forward (8192 rows x 4096, bf16), 2 / 4 / 8 54.8 / 57.5 / 57.3 us for both passes
+# (4096 x 2048, f32).
 CONV_UNITS, CONV_GRAD_UNITS = 8, 2
+# Blocks a multiprocessor of the norm: 2 / 4 / 6 / 16 70 / 71 / 77 / 80 us (8192 x 4096 bf16), backward 1 / 2 / 4 142 / 152 /
+# 170 us for both passes (4096 x 4096 bf16): every block sums its own share of the parameter gradients.
 NORM_UNITS, NORM_GRAD_UNITS = 2, 1
-TOKEN_ROWS = 4          # sequences of at most this many rows: the scan's token kernel
+# Sequences of at most this many rows go through the scan's token kernel.  4096 channels x 16 states, token kernel / walk:
+# 1 row 4.7 / 6.0 us (one sequence) and 26 / 73 us (128 sequences), 2 rows 6.0 / 6.0 and 41 / 75, 4 rows 8.3 / 5.9 and 72 / 77.
+TOKEN_ROWS = 2
+# Sequences up to this length are not split; a unit has at least SCAN_LEAST_ROWS rows (512 rows x 1024 channels in units
+# of 32 / 64 / 128: 20 / 24 / 37 us), and a split makes about SCAN_BLOCKS blocks (16384 x 1024: 592 / 1184 / 2368 220 / 212 / 214 us).
+SCAN_WHOLE_ROWS, SCAN_LEAST_ROWS, SCAN_BLOCKS = 96, 32, 148 * 8
 
 
 # ---- argument checks -------------------------------------------------------------------------
@@ -367,14 +379,18 @@ def scan_tile(n_states, backward=False):
     return 128 // lanes * (1 if backward else 2)
 
 
-def _scan_units(a, args, tiles, want):
-    """Splits the sequences into units of rows.  A block walks a unit row after row, so a batch of few channels
-    or one long sequence is split over time until there are ``want`` blocks; that computes every row's
-    decay twice (once for the units' ends).  Returns the sequences' first units and what to place."""
+def _scan_units(a, args, tiles, row, work, twice):
+    """Splits the sequences into units of rows, or not.  A block walks a unit row after row: unsplit, the longest
+    sequence takes ``row`` us a row however few blocks there are, and the whole batch ``work`` us a row and tile of
+    channels.  Split, the batch takes ``twice`` that (every row's decay is computed again for the units' ends) and
+    three launches.  The cheaper one is taken; measured on a B200, 4096 channels x 16 states, float32, unsplit / split:
+    2 x 1024 rows 147 / 119 us, 4 x 1024 178 / 217, 2 x 2048 289 / 221, 8 x 512 140 / 229; backward, 2048
+    channels: 2 x 512 rows 283 / 117, 8 x 256 188 / 214.  Returns the sequences' first units and what to place."""
     longest, total = max(int(a.lengths.max()), 1), int(a.lengths.sum())
     args.unit_rows = -(-longest // 32) * 32
-    if len(a.lengths) * tiles < want // 2 and longest > 128:
-        args.unit_rows = min(args.unit_rows, max(64, -(-total * tiles // (want * 32)) * 32))
+    whole = max(longest * row, total * tiles * work)
+    if longest > SCAN_WHOLE_ROWS and whole > twice * total * tiles * work + 2 * SCAN_LEAST_ROWS * row + 8:
+        args.unit_rows = min(args.unit_rows, max(SCAN_LEAST_ROWS, -(-total * tiles // (SCAN_BLOCKS * 32)) * 32))
     units = np.maximum(-(-a.lengths // args.unit_rows), 1)
     tokens = dict.fromkeys(("units", "ends", "sums"))
     tokens["units"], args.n_units = a.units(args.unit_rows)
@@ -437,7 +453,8 @@ def plan_selective_scan(queue, X, dt, A, B, C, Y, D=None, Z=None, dt_bias=None, 
     args.tokens = int(longest <= TOKEN_ROWS and not keep)
     launches, first_unit, tokens = 1, np.arange(len(a.lengths)), {}
     if not args.tokens:
-        first_unit, tokens = _scan_units(a, args, groups * -(-(a.channels // groups) // scan_tile(n)), 148 * 8)
+        first_unit, tokens = _scan_units(a, args, groups * -(-(a.channels // groups) // scan_tile(n)), 0.135, 4.2e-4,
+                                         2.2)
         launches = 3 if tokens["ends"] is not None else 1
     a.place(args, table=a.table(first, first_unit), keep=kept, **tokens)
     total = int(a.lengths.sum())
@@ -494,7 +511,7 @@ def plan_selective_scan_grad(queue, plan, dY, dX, ddt, dA, dB, dC, dD=None, dZ=N
     total = int(a.lengths.sum())
     args.total_rows = total
     tiles = -(-(a.channels // groups) // scan_tile(n, backward=True))
-    first_unit, tokens = _scan_units(a, args, groups * tiles, 148 * 8)
+    first_unit, tokens = _scan_units(a, args, groups * tiles, 0.5, 1.3e-3, 1.25)
     a.place(args, table=a.table(f["first"], np.cumsum(a.lengths) - a.lengths, first_unit, np.zeros_like(first_unit)),
             part_bc=a.scratch(tiles * total * 2 * width), part_a=a.scratch(args.n_units * a.channels * n),
             part_d=a.scratch(args.n_units * a.channels), part_s=a.scratch(args.n_units * a.channels), **tokens)
