@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, VEC ? 5 : 4) nb2_selective_scan_
 
   scan_clear_weights(stages, 2);  // the padding states' stay zero: only the real ones are written
   __syncthreads();
-  ScanWeights<VEC, T, S, R> weights;
+  ScanWeights<VEC, T, S, R> weights(n);
   ScanCopy<VEC, T, Stage> copy[NA];
   auto fetch = [&](Stage& st, int64_t from, int rows) {
     copy[0].load(st.in[0], dt + from * pt.stride, pt.stride, rows, l.width);

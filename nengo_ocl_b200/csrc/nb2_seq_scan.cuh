@@ -252,31 +252,29 @@ struct ScanWeights {
   static constexpr int kPer = VEC ? 16 / (int)sizeof(T) : 1;
   static constexpr int kCount = (R * 8 * S / kPer + SCAN_THREADS - 1) / SCAN_THREADS;
   SeqVecA<T, kPer> v[kCount];
-  // entry i of the thread: (row, B or C, first state); false past the tile
-  static __device__ __forceinline__ bool at(int i, int n, int& r, int& which, int& m) {
-    const int per = n / kPer, e = threadIdx.x + i * SCAN_THREADS;
-    r = e / (2 * per);
-    const int rest = e - r * 2 * per;
-    which = rest >= per;
-    m = (rest - which * per) * kPer;
-    return r < R;
+  int to[kCount];  // place of entry i in [R][B, C][4 S], -1 past the tile (the same for every tile)
+  __device__ __forceinline__ explicit ScanWeights(int n) {
+    const int per = n / kPer;
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      const int e = threadIdx.x + i * SCAN_THREADS, row = e / per, m = (e - row * per) * kPer;
+      to[i] = row < 2 * R ? row * 4 * S + m : -1;
+    }
   }
   __device__ __forceinline__ void load(const T* B, int64_t bs, const T* C, int64_t cs, int n, int rows) {
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
-      int r, which, m;
+      const int r = to[i] / (8 * S), m = to[i] % (4 * S);
       v[i].zero();
-      if (at(i, n, r, which, m) && r < rows) v[i].load((which ? C + r * cs : B + r * bs) + m);
+      if (to[i] >= 0 && r < rows) v[i].load((to[i] & (4 * S) ? C + r * cs : B + r * bs) + m);
     }
   }
   __device__ __forceinline__ void store(float (&bc)[R][2][4 * S], int n) const {
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) {
-      int r, which, m;
-      if (at(i, n, r, which, m))
+    for (int i = 0; i < kCount; ++i)
+      if (to[i] >= 0)
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) bc[r][which][m + e] = v[i][e];
-    }
+        for (int e = 0; e < kPer; ++e) (&bc[0][0][0])[to[i] + e] = v[i][e];
   }
 };
 

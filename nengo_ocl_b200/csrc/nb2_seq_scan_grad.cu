@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) nb2_scan_grad_ends_kernel(const 
   float total = 0.0f;
   scan_clear_weights(stages, 2);
   __syncthreads();
-  ScanWeights<VEC, T, S, R> weights;
+  ScanWeights<VEC, T, S, R> weights(n);
   ScanCopy<VEC, T, Stage> copy[NA];
   auto fetch = [&](Stage& st, int64_t from, int rows) {
     copy[0].load(st.in[0], dt + from * pt.stride, pt.stride, rows, l.width);
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 && VEC ? 4 : 3) nb2_selec
   float dD = 0.0f, dbias = 0.0f, h0[4];
   scan_clear_weights(stages, 2);
   __syncthreads();
-  ScanWeights<VEC, T, S, R> weights;
+  ScanWeights<VEC, T, S, R> weights(n);
   ScanCopy<VEC, T, Stage> copy[NA];
   auto fetch = [&](Stage& st, int64_t from, int rows) {
     copy[0].load(st.in[0], dt + from * pt.stride, pt.stride, rows, l.width);
@@ -352,9 +352,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 && VEC ? 4 : 3) nb2_selec
     if (tb > 0) arrive(stages[cur ^ 1]);
     __syncthreads();
     // the block's share of dB and dC: warps in order
-    for (int i = tid; i < rows * 2 * n; i += SCAN_THREADS) {
-      const int r = i / (2 * n), m = i - r * 2 * n;
-      const int col = m < n ? m : 4 * S + m - n;
+    for (int i = tid; i < rows * 8 * S; i += SCAN_THREADS) {
+      const int r = i / (8 * S), col = i % (8 * S), state = col % (4 * S), m = col < 4 * S ? state : n + state;
+      if (state >= n) continue;
       float sum = 0.0f;
 #pragma unroll
       for (int w = 0; w < SCAN_WARPS; ++w) sum += sm.red[r][w][col];

@@ -233,7 +233,7 @@ SCANS = [  # chan, n, groups, pad, lead, options
 
 
 @DTYPES
-@pytest.mark.parametrize("lengths", LENGTHS, ids=str)
+@pytest.mark.parametrize("lengths", LENGTHS + [[210, 0, 33]], ids=str)
 @pytest.mark.parametrize("chan,n,groups,pad,lead,options", SCANS)
 def test_selective_scan(queue, rng, dtype, lengths, chan, n, groups, pad, lead, options):
     s = Scan(queue, rng, lengths, chan, n, groups, dtype, pad, lead, **options)
@@ -250,7 +250,7 @@ def test_selective_scan(queue, rng, dtype, lengths, chan, n, groups, pad, lead, 
 
 
 @DTYPES
-@pytest.mark.parametrize("lengths", LENGTHS, ids=str)
+@pytest.mark.parametrize("lengths", LENGTHS + [[210, 0, 33]], ids=str)
 @pytest.mark.parametrize("chan,n,groups,pad,lead,options", SCANS)
 def test_selective_scan_grad(queue, rng, dtype, lengths, chan, n, groups, pad, lead, options):
     s = Scan(queue, rng, lengths, chan, n, groups, dtype, pad, lead, **options)
