@@ -323,35 +323,6 @@ __global__ void __launch_bounds__(256) nb2_conv_grad_sum_kernel(const float* par
   }
 }
 
-// Every block of a grid-stride loop owns 32 columns: eight interleaved runs over the parts, then their sum.
-__global__ void __launch_bounds__(256) nb2_seq_sum_parts_kernel(const float* part, int64_t n_parts, int64_t n, float* out) {
-  nb2_pdl_enter();
-  __shared__ float run[8][33];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  for (int64_t b = blockIdx.x; b * 32 < n; b += gridDim.x) {
-    const int64_t i = b * 32 + lane;
-    float s = 0.0f;
-    if (i < n)
-#pragma unroll 8
-      for (int64_t u = w; u < n_parts; u += 8) s += part[u * n + i];
-    run[w][lane] = s;
-    __syncthreads();
-    if (w == 0 && i < n) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int r = 0; r < 8; ++r) sum += run[r][lane];
-      out[i] = sum;
-    }
-    __syncthreads();
-  }
-}
-
-cudaError_t nb2_seq_sum_parts(cudaStream_t s, const float* part, int64_t n_parts, int64_t n, float* out) {
-  const int64_t blocks = (n + 31) / 32;
-  return nb2_launch(nb2_seq_sum_parts_kernel, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, s, part,
-                    n_parts, n, out);
-}
-
 template <typename K, typename A>
 static cudaError_t conv_run(K kernel, dim3 grid, int smem, cudaStream_t s, const A& a, int tiles) {
   if (smem > 48 * 1024) {

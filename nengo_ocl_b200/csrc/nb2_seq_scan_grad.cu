@@ -384,25 +384,56 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 && VEC ? 4 : 3) nb2_selec
   }
 }
 
-// dB and dC of every row: the channel tiles' shares added in order.
+// dB and dC of every row: the channel tiles' shares added in order.  A thread per value, rows of all sequences in one.
 template <typename T>
 __global__ void __launch_bounds__(256) nb2_scan_grad_bc_kernel(const nb2_selective_scan_grad_args a, int tiles) {
-  nb2_pdl_enter();
+  nb2_pdl_wait();
   const int n = a.n_states, wide = a.groups * 2 * n;
-  const int64_t all = a.total_rows * wide;
-  const int k = blockIdx.y;
-  const int64_t len = a.table[k], row0 = a.table[(size_t)28 * a.n_seq + k];
-  const ScanPlace pb = scan_place(a.table, a.n_seq, 8, k), pc = scan_place(a.table, a.n_seq, 9, k);
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < len * wide; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / wide;
-    const int rest = (int)(i - r * wide), group = rest / (2 * n), m = rest - group * 2 * n;
-    float sum = 0.0f;
+  const int64_t all = a.total_rows * wide, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= all) return;
+  float sum = 0.0f;
+#pragma unroll 16
+  for (int u = 0; u < tiles; ++u) sum += a.part_bc[u * all + i];
+  const int64_t row = i / wide;
+  const int rest = (int)(i - row * wide), group = rest / (2 * n), m = rest - group * 2 * n;
+  const int64_t* before = a.table + (size_t)28 * a.n_seq;  // rows of the sequences before each
+  int k = 0;
+  for (int span = a.n_seq; span > 1;) {  // the last sequence that begins at or before the row (and is not empty)
+    const int half = span / 2;
+    if (before[k + half] <= row) k += half, span -= half;
+    else span = half;
+  }
+  const ScanPlace p = scan_place(a.table, a.n_seq, m < n ? 8 : 9, k);
+  ((T*)(m < n ? a.dB : a.dC))[p.start + (row - before[k]) * p.stride + group * n + (m < n ? m : m - n)] = nb2_from_float<T>(sum);
+}
+
+// Gradients of A, D and dt_bias: the units' shares added in order within eight interleaved runs.  A block owns 32
+// columns of [channels x n_states | channels | channels].
+__global__ void __launch_bounds__(256) nb2_scan_grad_sum_kernel(const nb2_selective_scan_grad_args a) {
+  nb2_pdl_wait();
+  __shared__ float run[8][33];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t states = (int64_t)a.channels * a.n_states, i = (int64_t)blockIdx.x * 32 + lane;
+  const float* part = nullptr;
+  float* out = nullptr;
+  int64_t n = a.channels, at = i;
+  if (i < states)
+    part = a.part_a, out = a.dA, n = states;
+  else if (i < states + a.channels)
+    part = a.part_d, out = a.dD, at = i - states;
+  else if (i < states + 2 * a.channels)
+    part = a.part_s, out = a.ddt_bias, at = i - states - a.channels;
+  float s = 0.0f;
+  if (out)
 #pragma unroll 8
-    for (int u = 0; u < tiles; ++u) sum += a.part_bc[u * all + (row0 + r) * wide + rest];
-    if (m < n)
-      ((T*)a.dB)[pb.start + r * pb.stride + group * n + m] = nb2_from_float<T>(sum);
-    else
-      ((T*)a.dC)[pc.start + r * pc.stride + group * n + m - n] = nb2_from_float<T>(sum);
+    for (int u = w; u < a.n_units; u += 8) s += part[u * n + at];
+  run[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && out) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) sum += run[r][lane];
+    out[at] = sum;
   }
 }
 
@@ -432,19 +463,16 @@ extern "C" int nb2_selective_scan_grad(void* stream, const nb2_selective_scan_gr
   if (int e = scan_check(a)) return e;
   NB2_REQUIRE(a.dy && a.dx && a.ddt && a.dB && a.dC && a.dA && a.keep && a.part_bc && a.part_a, "null pointer");
   NB2_REQUIRE((!a.dz || a.z) && (!a.dD || (a.D && a.part_d)) && (!a.ddt_bias || (a.dt_bias && a.part_s)), "gradients");
-  NB2_REQUIRE(a.n_seq <= 65535, "too many sequences");
   if (int e = scan_check_units(a)) return e;
   cudaStream_t s = nb2_stream(stream);
   const int tiles = scan_tiles(a.channels, a.groups, SCAN_THREADS / scan_lanes(a.n_states));
   NB2_SEQ_DTYPE(a.dtype, SCAN_BY_LANES(scan_lanes(a.n_states), scan_grad_launch));
   if (a.total_rows > 0) {
-    const int64_t wide = (a.total_rows * a.groups * 2 * a.n_states + 255) / 256;
-    const int64_t per = (wide + a.n_seq - 1) / a.n_seq;
-    const dim3 grid((unsigned)(per < 8192 ? per : 8192), (unsigned)a.n_seq);
-    NB2_SEQ_DTYPE(a.dtype, NB2_CUDA(nb2_launch(nb2_scan_grad_bc_kernel<T>, grid, dim3(256), 0, s, a, tiles)));
+    const int64_t blocks = (a.total_rows * a.groups * 2 * a.n_states + 255) / 256;
+    NB2_REQUIRE(blocks < (1ll << 31), "too many rows");
+    NB2_SEQ_DTYPE(a.dtype, NB2_CUDA(nb2_launch(nb2_scan_grad_bc_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, a, tiles)));
   }
-  NB2_CUDA(nb2_seq_sum_parts(s, a.part_a, a.n_units, (int64_t)a.channels * a.n_states, a.dA));
-  if (a.dD) NB2_CUDA(nb2_seq_sum_parts(s, a.part_d, a.n_units, a.channels, a.dD));
-  if (a.ddt_bias) NB2_CUDA(nb2_seq_sum_parts(s, a.part_s, a.n_units, a.channels, a.ddt_bias));
+  const int64_t columns = (int64_t)a.channels * (a.n_states + 2);
+  NB2_CUDA(nb2_launch(nb2_scan_grad_sum_kernel, dim3((unsigned)((columns + 31) / 32)), dim3(256), 0, s, a));
   return NB2_OK;
 }

@@ -116,6 +116,3 @@ __device__ __forceinline__ float nb2_silu_slope(float v) {
       __VA_ARGS__;                                      \
     }                                                   \
   } while (0)
-
-// out[i] = sum over p of part[p * n + i], p in order: the same result for every run
-cudaError_t nb2_seq_sum_parts(cudaStream_t s, const float* part, int64_t n_parts, int64_t n, float* out);

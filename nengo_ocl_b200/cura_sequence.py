@@ -516,7 +516,7 @@ def plan_selective_scan_grad(queue, plan, dY, dX, ddt, dA, dB, dC, dD=None, dZ=N
             part_bc=a.scratch(tiles * total * 2 * width), part_a=a.scratch(args.n_units * a.channels * n),
             part_d=a.scratch(args.n_units * a.channels), part_s=a.scratch(args.n_units * a.channels), **tokens)
     return _make_plan(queue, "cura_selective_scan_grad", "nb2_selective_scan_grad", args, a.kept,
-                      len(a.lengths) * a.channels, 5 + 2 * bool(args.ends), tag, total * a.channels * (19 * n + 30), moved)
+                      len(a.lengths) * a.channels, 3 + 2 * bool(args.ends), tag, total * a.channels * (19 * n + 30), moved)
 
 
 # ---- norms around a block --------------------------------------------------------------------
