@@ -3,6 +3,10 @@
 //   pre[t] = bias + sum_j w[j] x[t - W + 1 + j],   y = pre or pre sigmoid(pre)
 //   dpre = dy * act'(pre),  dx[p] = sum_j w[j] dpre[p + W - 1 - j],  dw[j] = sum_t dpre[t] x[t - W + 1 + j]
 // Rows before the first one come from the state, which is also a sequence's last W - 1 rows.
+//
+// Memory would allow 20 us for 8192 rows x 4096 channels in bfloat16; the kernel takes 40: with 4 taps and the silu a value
+// is 16 instructions, and the window and weights of four channels leave 20 warps to a multiprocessor.  Eight
+// channels to a thread 47 us, weights read from memory by each thread 54, one row at a time 81.
 #include "nb2_sequence.cuh"
 
 #define CONV_THREADS 128

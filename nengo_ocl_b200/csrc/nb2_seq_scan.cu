@@ -8,31 +8,43 @@
 //
 // A tile of R rows is worked in three phases, each a warp's own: its lanes prepare (s, s x) of the tile's rows
 // for their channels, walk the rows through the states, and finish the outputs.
+//
+// Bound by the special function unit: n + 4 results a row and channel at 16 a cycle and multiprocessor, 25 us for
+// 4096 rows x 1024 channels x 16 states and walk where memory needs 10 (float32).  Measured (B200): 48 x 256 rows x 4096
+// channels 326 us, 0.7 of the unit busy (231 us of it at full rate); 4097 rows of 4 uneven prompts, split, 226 us. Six
+// blocks a multiprocessor (80 registers) against five and four: 226 / 231 / 231 us; rows copied element by
+// element need more registers: four.
 #define SCAN_P 2
 #define SCAN_TOKEN_BLOCKS 16
 template <typename T, int S, bool VEC, bool ENDS>
-__global__ void __launch_bounds__(SCAN_THREADS, VEC ? 5 : 4) nb2_selective_scan_kernel(const nb2_selective_scan_args a) {
+__global__ void __launch_bounds__(SCAN_THREADS, VEC ? 6 : 4) nb2_selective_scan_kernel(const nb2_selective_scan_args a) {
   constexpr int P = SCAN_P, R = NB2_SCAN_KEEP, RB = S < 4 ? S : 4;
   constexpr int NA = 3;
   using Stage = ScanStage<T, S, P, R, NA>;
   extern __shared__ __align__(16) char smem_raw[];
   Stage* stages = reinterpret_cast<Stage*>(smem_raw);
   ScanRows<S, P, R>& ready = *reinterpret_cast<ScanRows<S, P, R>*>(smem_raw + 2 * sizeof(Stage));
+  enum { kDt, kX, kZ, kB, kC, kY, kArrays };
+  __shared__ ScanArray arrays[kArrays];
   nb2_pdl_wait();
   const ScanLane<S, P> l(a.channels, a.groups, a.units);
   const int n = a.n_states;
   const int64_t len = a.table[l.k], t0 = l.first, t1 = min(t0 + a.unit_rows, len);
   if (ENDS && t1 == len) return;  // nothing starts from the last unit's end
   const int64_t nk = a.n_seq;
-  const ScanPlace px = scan_place(a.table, nk, 0, l.k), pt = scan_place(a.table, nk, 1, l.k),
-                  pb = scan_place(a.table, nk, 2, l.k), pc = scan_place(a.table, nk, 3, l.k),
-                  py = scan_place(a.table, nk, 4, l.k), pz = scan_place(a.table, nk, 5, l.k);
-  const T* x = (const T*)a.x + px.start + t0 * px.stride + l.c0;
-  const T* dt = (const T*)a.dt + pt.start + t0 * pt.stride + l.c0;
-  const T* z = !ENDS && a.z ? (const T*)a.z + pz.start + t0 * pz.stride + l.c0 : nullptr;
-  const T* B = (const T*)a.B + pb.start + t0 * pb.stride + (int64_t)l.group * n;
-  const T* C = (const T*)a.C + pc.start + t0 * pc.stride + (int64_t)l.group * n;
-  T* y = (T*)a.y + py.start + t0 * py.stride + l.c0 + l.in_block;
+  if (threadIdx.x < kArrays) {
+    const int field[kArrays] = {1, 0, 5, 2, 3, 4};
+    const void* const base[kArrays] = {a.dt, a.x, a.z, a.B, a.C, a.y};
+#pragma unroll
+    for (int q = 0; q < kArrays; ++q)
+      if (threadIdx.x == q) {
+        const ScanPlace p = scan_place(a.table, nk, field[q], l.k);
+        const int64_t column = q == kB || q == kC ? (int64_t)l.group * n : l.c0;
+        arrays[q].p = (char*)base[q] + (p.start + t0 * p.stride + column) * (int64_t)sizeof(T);
+        arrays[q].stride = p.stride;
+      }
+  }
+  const bool gate = !ENDS && a.z;
   f32x2 A2[P][2], h[P][2];
   float D[P], bias[P], total[P];
 #pragma unroll
@@ -63,17 +75,20 @@ __global__ void __launch_bounds__(SCAN_THREADS, VEC ? 5 : 4) nb2_selective_scan_
   ScanWeights<VEC, T, S, R> weights(n);
   ScanCopy<VEC, T, Stage> copy[NA];
   auto fetch = [&](Stage& st, int64_t from, int rows) {
-    copy[0].load(st.in[0], dt + from * pt.stride, pt.stride, rows, l.width);
-    copy[1].load(st.in[1], x + from * px.stride, px.stride, rows, l.width);
-    if (z)
-      copy[2].load(st.in[2], z + from * pz.stride, pz.stride, rows, l.width);
-    weights.load(B + from * pb.stride, pb.stride, C + from * pc.stride, pc.stride, n, rows);
+#pragma unroll
+    for (int q = 0; q < NA; ++q)
+      if (q != kZ || gate) {
+        const ScanArray r = arrays[q];
+        copy[q].load(st.in[q], (const T*)r.p + from * r.stride, r.stride, rows, l.width);
+      }
+    const ScanArray b = arrays[kB], c = arrays[kC];
+    weights.load((const T*)b.p + from * b.stride, b.stride, (const T*)c.p + from * c.stride, c.stride, n, rows);
   };
   auto arrive = [&](Stage& st) {
     weights.store(st.bc, n);
 #pragma unroll
     for (int i = 0; i < NA; ++i)
-      if (i < 2 || z) copy[i].store(st.in[i]);
+      if (i != kZ || gate) copy[i].store(st.in[i]);
   };
   const int64_t all = t1 - t0;
   if (all > 0) {
@@ -166,8 +181,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, VEC ? 5 : 4) nb2_selective_scan_
         }
       }
     }
-    if (!ENDS)
-      scan_switch(z != nullptr, [&](auto gated) {
+    if (!ENDS) {
+      const ScanArray to = arrays[kY];
+      T* y = (T*)to.p + mine;
+      scan_switch(gate, [&](auto gated) {
 #pragma unroll
         for (int q = 0; q < R / RB; ++q) {
           const int r = q * RB + j;
@@ -179,9 +196,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, VEC ? 5 : 4) nb2_selective_scan_
             o[p] = fmaf(D[p], xv[p], out[q][p]);
             if (decltype(gated)::value) o[p] *= zv[p] * nb2_sigmoid(zv[p]);
           }
-          if (r < rows) scan_put<VEC, T, P>(y + (tb + r) * py.stride, o, stores);
+          if (r < rows) scan_put<VEC, T, P>(y + (tb + r) * to.stride, o, stores);
         }
       });
+    }
     if (next > 0) arrive(stages[cur ^ 1]);
   }
 #pragma unroll
@@ -248,7 +266,9 @@ cudaError_t nb2_scan_join(cudaStream_t s, ScanJoin j) {
 
 // Single tokens and a few rows: the states are most of the traffic, one read and one write of each.  A block keeps
 // its channels' parameters and takes one sequence after the other, the next one's state and first row on their
-// way while it works.
+// way while it works.  Bound by memory, 8 bytes a state; measured 50 us = 2.9 TB/s for 256 tokens x 4096 channels x 16
+// states, with the table read from memory per sequence 58, one block per sequence and 128 channels 81; eight blocks a
+// multiprocessor (64 registers) against six: 51 / 59 us; channels of a lane 1 / 2 / 4: 60 / 51 / 74 us.
 constexpr int kTokenUnroll = 2;  // channels of a lane, SCAN_THREADS / S apart
 constexpr int kTokenSequences = 64, kTokenFields = 17;  // of a block; of the table: the length and eight (start, stride)
 template <typename T, int S>

@@ -13,6 +13,7 @@
 #define SCAN_WARPS 4
 #define SCAN_THREADS (32 * SCAN_WARPS)
 #define LOG2E 1.4426950408889634f
+#define LN2 0.6931471805599453f
 
 static int scan_lanes(int n_states) {
   int s = 1;
@@ -156,6 +157,12 @@ __device__ __forceinline__ void scan_cp_async(void* smem, const void* gmem, int 
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(s), "l"(gmem) : "memory");
 }
 __device__ __forceinline__ void scan_cp_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Where an array's rows of the unit begin: in shared memory, since nine of them would fill 36 registers (backward), six 24.
+struct ScanArray {
+  char* p;
+  int64_t stride;
+};
 
 // What a block stages in shared memory: R rows of its channels of NA arrays in their own type, and the
 // rows' weights B, C in float32 (converted once for all its channels), padded with zeros to 4 S states.

@@ -8,12 +8,19 @@
 // and states from the kept state into registers, then goes back through its rows.  Units as in the forward
 // pass, run through from the last: nb2_scan_grad_ends_kernel leaves the gradient that each would hand on if it
 // received zero.
+//
+// Bound by shared-memory words and issue slots: a lane reads 26 words a row (B and C twice, the prepared rows) and the
+// sums over channels and states are 9 shuffles.  Measured (B200, 2 x 2048 rows x 2048 channels x 16 states, float32): both
+// passes 427 us, of which this walk about 230; 16 x 512 rows 654.  Four blocks a multiprocessor against three and five:
+// 427 / 456 / 477 us; above 32 states three: 543 against 617 with four.  Two channels to a lane spill: 466.
+enum ScanGradArrays { kDt, kX, kDy, kZ, kB, kC, kDx, kDdt, kDz, kArrays };
 template <int S>
 struct ScanGradSmem {
   static constexpr int R = NB2_SCAN_KEEP;
+  ScanArray arrays[kArrays];
   ScanRows<S, 1, R> ready;
   float dp[R][ScanRows<S, 1, R>::kPitch];
-  float4 sums[R][SCAN_THREADS / S];  // over the states: g B, g a h[t-1] A, C h
+  float4 sums[R][SCAN_THREADS / S];  // over the states: g B, g a h[t-1] A log2(e), C h
   alignas(16) float red[R][SCAN_WARPS][8 * S];  // dB, dC of a row: a warp's channels added
 };
 
@@ -142,7 +149,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) nb2_scan_grad_ends_kernel(const 
 }
 
 template <typename T, int S, bool VEC>
-__global__ void __launch_bounds__(SCAN_THREADS, S < 16 && VEC ? 4 : 3) nb2_selective_scan_grad_kernel(const nb2_selective_scan_grad_args a) {
+__global__ void __launch_bounds__(SCAN_THREADS, S < 16 ? 4 : 3) nb2_selective_scan_grad_kernel(const nb2_selective_scan_grad_args a) {
   constexpr int R = NB2_SCAN_KEEP, RB = S < 4 ? S : 4;
   constexpr int NA = 4;
   using Stage = ScanStage<T, S, 1, R, NA>;
@@ -154,28 +161,24 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 && VEC ? 4 : 3) nb2_selec
   const ScanLane<S, 1> l(a.channels, a.groups, a.units);
   const int n = a.n_states, c = l.channel(0), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t len = a.table[l.k], t0 = l.first, t1 = min(t0 + a.unit_rows, len), nk = a.n_seq;
-  const ScanPlace px = scan_place(a.table, nk, 0, l.k), pt = scan_place(a.table, nk, 1, l.k),
-                  pb = scan_place(a.table, nk, 2, l.k), pc = scan_place(a.table, nk, 3, l.k),
-                  pz = scan_place(a.table, nk, 4, l.k), pdy = scan_place(a.table, nk, 5, l.k),
-                  pdx = scan_place(a.table, nk, 6, l.k), pdt = scan_place(a.table, nk, 7, l.k),
-                  pdz = scan_place(a.table, nk, 10, l.k);
-  const T* x = (const T*)a.x + px.start + t0 * px.stride + l.c0;
-  const T* dt = (const T*)a.dt + pt.start + t0 * pt.stride + l.c0;
-  const T* z = a.z ? (const T*)a.z + pz.start + t0 * pz.stride + l.c0 : nullptr;
-  const T* dy = (const T*)a.dy + pdy.start + t0 * pdy.stride + l.c0;
-  const T* B = (const T*)a.B + pb.start + t0 * pb.stride + (int64_t)l.group * n;
-  const T* C = (const T*)a.C + pc.start + t0 * pc.stride + (int64_t)l.group * n;
-  T* dx = (T*)a.dx + pdx.start + t0 * pdx.stride + c;
-  T* ddt = (T*)a.ddt + pdt.start + t0 * pdt.stride + c;
-  T* dz = a.dz ? (T*)a.dz + pdz.start + t0 * pdz.stride + c : nullptr;
+  if (tid < kArrays) {
+    const int field[kArrays] = {1, 0, 5, 4, 2, 3, 6, 7, 10};
+    const void* const base[kArrays] = {a.dt, a.x, a.dy, a.z, a.B, a.C, a.dx, a.ddt, a.dz};
+#pragma unroll
+    for (int q = 0; q < kArrays; ++q)
+      if (tid == q) {
+        const ScanPlace p = scan_place(a.table, nk, field[q], l.k);
+        const int64_t column = q == kB || q == kC ? (int64_t)l.group * n : l.c0;
+        sm.arrays[q].p = (char*)base[q] + (p.start + t0 * p.stride + column) * (int64_t)sizeof(T);
+        sm.arrays[q].stride = p.stride;
+      }
+  }
+  const bool gate = a.z != nullptr, dgate = a.dz != nullptr;
   const float* keep = a.keep + ((a.table[27 * nk + l.k] + t0 / R) * a.channels + c) * n;
   const int64_t row0 = a.table[28 * nk + l.k] + t0;
-  f32x2 A2[2], A[2], carry[2], dA[2] = {0, 0};
+  f32x2 A2[2], carry[2], dA[2] = {0, 0};
   float v[4];
   scan_rates(a.A + (int64_t)c * n, l.n0, n, A2);
-  scan_load4(a.A + (int64_t)c * n, l.n0, n, 0, v);
-  A[0] = pack2(v[0], v[1]);
-  A[1] = pack2(v[2], v[3]);
 #pragma unroll
   for (int m = 0; m < 4; ++m) v[m] = 0.0f;
   if (l.valid(0)) {
@@ -197,18 +200,24 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 && VEC ? 4 : 3) nb2_selec
   ScanWeights<VEC, T, S, R> weights(n);
   ScanCopy<VEC, T, Stage> copy[NA];
   auto fetch = [&](Stage& st, int64_t from, int rows) {
-    copy[0].load(st.in[0], dt + from * pt.stride, pt.stride, rows, l.width);
-    copy[1].load(st.in[1], x + from * px.stride, px.stride, rows, l.width);
-    copy[2].load(st.in[2], dy + from * pdy.stride, pdy.stride, rows, l.width);
-    if (z)
-      copy[3].load(st.in[3], z + from * pz.stride, pz.stride, rows, l.width);
-    weights.load(B + from * pb.stride, pb.stride, C + from * pc.stride, pc.stride, n, rows);
+#pragma unroll
+    for (int q = 0; q < NA; ++q)
+      if (q != kZ || gate) {
+        const ScanArray r = sm.arrays[q];
+        copy[q].load(st.in[q], (const T*)r.p + from * r.stride, r.stride, rows, l.width);
+      }
+    const ScanArray b = sm.arrays[kB], c = sm.arrays[kC];
+    weights.load((const T*)b.p + from * b.stride, b.stride, (const T*)c.p + from * c.stride, c.stride, n, rows);
     scan_load4(keep + from / R * a.channels * n, l.n0, n, n % 4 == 0, h0);
   };
   auto arrive = [&](Stage& st) {
     weights.store(st.bc, n);
 #pragma unroll
     for (int i = 0; i < NA; ++i) copy[i].store(st.in[i]);
+  };
+  auto put = [&](int q, int64_t row, float v) {
+    const ScanArray r = sm.arrays[q];
+    ((T*)r.p)[row * r.stride + mine] = nb2_from_float<T>(v);
   };
   const int64_t all = t1 - t0, last = (all - 1) / R * R;
   if (all > 0) {
@@ -224,7 +233,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 && VEC ? 4 : 3) nb2_selec
     const f32x2 start[2] = {pack2(h0[0], h0[1]), pack2(h0[2], h0[3])};
     if (tb > 0) fetch(stages[cur ^ 1], tb - R, R);
     scan_switch(a.softplus, [&](auto soft) {
-      scan_switch(z != nullptr, [&](auto gated) {
+      scan_switch(gate, [&](auto gated) {
 #pragma unroll
         for (int r0 = 0; r0 < R; r0 += RB) {
           const int r = r0 + j;
@@ -300,7 +309,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 && VEC ? 4 : 3) nb2_selec
           float lo, hi;
           unpack2(fma2(g1, b.y, mul2(g0, b.x)), lo, hi);
           pu[i] = lo + hi;
-          unpack2(fma2(q1, A[1], mul2(q0, A[0])), lo, hi);
+          unpack2(fma2(q1, A2[1], mul2(q0, A2[0])), lo, hi);
           pe[i] = lo + hi;
           unpack2(fma2(cw.y, h1, mul2(cw.x, h0)), lo, hi);
           ps[i] = lo + hi;
@@ -328,21 +337,21 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 && VEC ? 4 : 3) nb2_selec
     }
     __syncwarp();
     scan_switch(a.softplus, [&](auto soft) {
-      scan_switch(dz != nullptr, [&](auto gated) {
+      scan_switch(dgate, [&](auto gated) {
 #pragma unroll
         for (int r0 = 0; r0 < R; r0 += RB) {
           const int r = r0 + j;
           const float raw = nb2_to_float(st.in[0][r][mine]) + bias, xv = nb2_to_float(st.in[1][r][mine]);
           const float4 sum = sm.sums[r][mine];
           const float dp = sm.dp[r][mine], u = sum.x;
-          float ds = fmaf(xv, u, sum.y), gz = 0.0f;
+          float ds = fmaf(xv, u, sum.y * LN2), gz = 0.0f;
           if (decltype(soft)::value) ds *= nb2_sigmoid(raw);
           if (decltype(gated)::value)
             gz = nb2_to_float(st.in[2][r][mine]) * fmaf(D, xv, sum.z) * nb2_silu_slope(nb2_to_float(st.in[3][r][mine]));
           if (r < rows && stores) {
-            dx[(tb + r) * pdx.stride] = nb2_from_float<T>(fmaf(D, dp, sm.ready.sx[r][mine].x * u));
-            ddt[(tb + r) * pdt.stride] = nb2_from_float<T>(ds);
-            if (decltype(gated)::value) dz[(tb + r) * pdz.stride] = nb2_from_float<T>(gz);
+            put(kDx, tb + r, fmaf(D, dp, sm.ready.sx[r][mine].x * u));
+            put(kDdt, tb + r, ds);
+            if (decltype(gated)::value) put(kDz, tb + r, gz);
             dD = fmaf(dp, xv, dD);
             dbias += ds;
           }
