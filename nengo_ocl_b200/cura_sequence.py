@@ -144,10 +144,10 @@ class _Arguments:
             raise ValueError("%s: the items' rows differ from those expected" % name)
         if (ra.shape1s != columns).any():
             raise ValueError("%s: %d columns are expected" % (name, columns))
-        starts, strides = ra.starts.astype(np.int64), ra.stride0s.astype(np.int64)
+        starts, strides = ra.index64("starts"), ra.index64("stride0s")
         rows = np.broadcast_to(lengths, starts.shape)
         strides = np.where(rows > 1, strides, columns)
-        if columns > 1 and ((ra.stride1s != 1) & (rows > 0)).any():
+        if columns > 1 and ((ra.index64("stride1s") != 1) & (rows > 0)).any():
             raise NotImplementedError("%s: channels must lie next to each other (stride1 == 1)" % name)
         if (strides < 0).any():
             raise NotImplementedError("%s: rows in reverse order" % name)

@@ -12,6 +12,10 @@ Same Python semantics as the reference's ``CLRaggedArray``
   buffer; ``clra[int] = value`` -> contiguous write, or read-modify-write of
   the bounding region for a discontiguous view (lines 256-299);
 * ``to_host()`` -> host ``RaggedArray`` of the whole buffer.
+
+Starts and strides may be anything up to 64 bits (``index64``): a buffer of more than 2^31 elements is
+a few GB.  The int32 arrays are what 32-bit index tables are built from; where a value does not fit,
+reading them raises ``OverflowError``.
 """
 
 from io import StringIO
@@ -39,7 +43,7 @@ def to_host(queue, darray, dtype, start, shape, elemstrides):
 
 
 class _LazyIndex:
-    """Descriptor pair: host int32 array + lazily uploaded device twin."""
+    """Descriptor pair: host int32 array + lazily uploaded device twin; the values themselves in 64 bits."""
 
     def __init__(self, name):
         self.name = name
@@ -50,12 +54,18 @@ class _LazyIndex:
     def __get__(self, obj, objtype=None):
         if obj is None:
             return self
-        return obj.__dict__["_" + self.name]
+        arr = obj.__dict__["_" + self.name]
+        if arr is None:
+            raise OverflowError("%s do not fit in 32 bits" % self.name)
+        return arr
 
     def __set__(self, obj, values):
-        arr = np.array(values, dtype=np.int32)
+        wide = np.array(values, dtype=np.int64)
+        wide.setflags(write=False)
+        arr = wide.astype(np.int32)
         arr.setflags(write=False)
-        obj.__dict__["_" + self.name] = arr
+        obj.__dict__["_wide_" + self.name] = wide
+        obj.__dict__["_" + self.name] = arr if np.array_equal(arr, wide) else None
         obj.__dict__.pop("_cl_" + self.name, None)
         obj.__dict__["_sizes"] = None
 
@@ -96,10 +106,14 @@ class CUDARaggedArray:
         self.names = names
         return self
 
+    def index64(self, name):
+        """``starts``, ``stride0s`` ... in 64 bits, whatever their values."""
+        return self.__dict__["_wide_" + name]
+
     def _device_index(self, name):
         key = "_cl_" + name
         if key not in self.__dict__:
-            self.__dict__[key] = to_device(self.queue, self.__dict__["_" + name])
+            self.__dict__[key] = to_device(self.queue, getattr(self, name))
         return self.__dict__[key]
 
     cl_starts = property(lambda self: self._device_index("starts"))
@@ -123,7 +137,7 @@ class CUDARaggedArray:
     @names.setter
     def names(self, names):
         if names is None:
-            names = [""] * len(self.starts)
+            names = [""] * len(self)
         self._names = tuple(names)
 
     @property
@@ -149,7 +163,7 @@ class CUDARaggedArray:
         self.cl_buf = to_device(self.queue, buf)
 
     def __len__(self):
-        return len(self.starts)
+        return len(self.index64("starts"))
 
     def __str__(self):
         out = StringIO()
@@ -163,9 +177,9 @@ class CUDARaggedArray:
         if is_iterable(item) or isinstance(item, slice):
             return self.getitem_device(item)
         item = int(item)
-        buf = to_host(self.queue, self.cl_buf, self.dtype, self.starts[item],
+        buf = to_host(self.queue, self.cl_buf, self.dtype, self.index64("starts")[item],
                       (self.shape0s[item], self.shape1s[item]),
-                      (self.stride0s[item], self.stride1s[item]))
+                      (self.index64("stride0s")[item], self.index64("stride1s")[item]))
         buf.setflags(write=False)
         return buf
 
@@ -175,14 +189,14 @@ class CUDARaggedArray:
         if is_iterable(item):
             item = np.asarray([int(i) for i in item], dtype=np.intp)
             return CUDARaggedArray.from_buffer(
-                self.queue, self.cl_buf, self.starts[item], self.shape0s[item], self.shape1s[item],
-                self.stride0s[item], self.stride1s[item], names=[self.names[i] for i in item])
+                self.queue, self.cl_buf, self.index64("starts")[item], self.shape0s[item], self.shape1s[item],
+                self.index64("stride0s")[item], self.index64("stride1s")[item], names=[self.names[i] for i in item])
         item = int(item)
         isz = self.dtype.itemsize
         arr = DeviceArray(self.queue, (self.shape0s[item], self.shape1s[item]), self.dtype,
                           data=self.cl_buf.base_data,
-                          offset=self.cl_buf.offset + int(self.starts[item]) * isz, base=self.cl_buf)
-        arr.strides = (int(self.stride0s[item]) * isz, int(self.stride1s[item]) * isz)
+                          offset=self.cl_buf.offset + int(self.index64("starts")[item]) * isz, base=self.cl_buf)
+        arr.strides = (int(self.index64("stride0s")[item]) * isz, int(self.index64("stride1s")[item]) * isz)
         return arr
 
     def __setitem__(self, item, new_value):
@@ -190,8 +204,8 @@ class CUDARaggedArray:
             raise NotImplementedError("assigning to several items at once is not supported")
         item = int(item)
         m, n = int(self.shape0s[item]), int(self.shape1s[item])
-        sm, sn = int(self.stride0s[item]), int(self.stride1s[item])
-        start = int(self.starts[item])
+        sm, sn = int(self.index64("stride0s")[item]), int(self.index64("stride1s")[item])
+        start = int(self.index64("starts")[item])
         if m * n == 0:
             return
         if self.dtype == bfloat16:
@@ -220,8 +234,8 @@ class CUDARaggedArray:
 
     def to_host(self):
         """Copy the whole object to a host RaggedArray."""
-        return RaggedArray.from_buffer(self.buf, self.starts, self.shape0s, self.shape1s,
-                                       self.stride0s, self.stride1s, names=self.names)
+        return RaggedArray.from_buffer(self.buf, self.index64("starts"), self.shape0s, self.shape1s,
+                                       self.index64("stride0s"), self.index64("stride1s"), names=self.names)
 
 
 # The reference's name, so planning code written against it imports unchanged.

@@ -22,7 +22,10 @@ _DTYPES = (np.dtype(np.float32), np.dtype(np.int32), np.dtype(np.float16), bfloa
 
 
 def _index_array(values):
-    arr = np.array(values, dtype=np.int32)
+    wide = np.array(values, dtype=np.int64)
+    arr = wide.astype(np.int32)
+    if not np.array_equal(arr, wide):
+        raise OverflowError("indices past 2^31 elements")
     arr.setflags(write=False)
     return arr
 

@@ -415,3 +415,55 @@ def test_oracle_steps_equal_whole_sequences():
     y, end = S.selective_scan(rows["conv0"], rows["dt0"], get("A"), rows["B0"], rows["C0"], get("D"), None, get("dt_bias"), True)
     # (the state is rounded to float32 after every step: 12 half steps)
     assert np.allclose(y, rows["scanned0"], rtol=1e-5, atol=1e-5) and np.allclose(end, ora[state], rtol=1e-5, atol=1e-6)
+
+
+# ---- places past 2^31 elements -------------------------------------------------------------------
+def _table(plan, args=None):
+    """The launch's table [fields][sequences] as it was uploaded (the stand-in's memory is the host's)."""
+    args = args or plan.full_args[0]
+    fields = {"nb2_causal_conv_args": 9, "nb2_residual_norm_args": 11, "nb2_selective_scan_args": 19}[type(args).__name__]
+    words = ctypes.cast(args.table, ctypes.POINTER(ctypes.c_int64))
+    return np.array([words[i] for i in range(fields * args.n_seq)]).reshape(fields, args.n_seq)
+
+
+def _far(queue, starts, rows, columns, pitch, size=2 ** 35, address=1 << 40, dtype=np.float32):
+    """Items of a buffer that is nowhere (nothing is launched): only its address and size are used."""
+    k = len(starts)
+    return CUDARaggedArray.from_buffer(queue, DeviceArray(queue, (size,), dtype, data=address), starts, [rows] * k,
+                                       [columns] * k, [pitch] * k, [1] * k)
+
+
+@pytest.mark.parametrize("start", [2 ** 31, 2 ** 31 + 8, 2 ** 32 + 64, 2 ** 33 + 2 ** 31])
+@pytest.mark.parametrize("listed", [False, True])
+def test_starts_and_strides_past_32_bits_reach_the_launch(fake_queue, start, listed):
+    q = fake_queue
+    starts = [start, 64]
+    x = _far(q, starts if listed else np.array(starts, np.int64), 2, 8, 2 ** 32 + 16)
+    y = _far(q, np.array([64, start], np.int64), 2, 8, 2 ** 33 + 16, address=1 << 42)
+    pool = _far(q, np.array([start, 2 * start]), 8, 4, 4, address=1 << 43)
+    small = _rows(q, [2, 2], 4)
+    plan = seq.plan_selective_scan(q, x, _rows(q, [2, 2], 8), DeviceArray(q, (8, 4), np.float32), small, small, y,
+                                   state=pool, new_state=pool)
+    t = _table(plan)
+    assert t[1].tolist() == starts and t[2].tolist() == [2 ** 32 + 16] * 2
+    assert t[9].tolist() == [64, start] and t[10].tolist() == [2 ** 33 + 16] * 2
+    assert t[13].tolist() == t[15].tolist() == [start, 2 * start]
+    assert _table(seq.plan_residual_norm(q, x, H=y))[1].tolist() == starts
+    # a selection of items keeps them
+    assert _table(seq.plan_residual_norm(q, x[[1, 0]], H=y[[1, 0]]))[1].tolist() == starts[::-1]
+    assert len(x) == 2 and x[1:].index64("starts").tolist() == [64]
+
+
+def test_places_past_32_bits_are_not_handed_to_32_bit_tables(fake_queue):
+    """What only takes int32 index tables gets an error, not the place's lower half."""
+    x = _far(fake_queue, np.array([2 ** 32 + 64]), 2, 8, 8)
+    for name in ("starts", "cl_starts"):
+        with pytest.raises(OverflowError, match="starts"):
+            getattr(x, name)
+    assert x.stride0s.dtype == np.int32 and x.stride0s.tolist() == [8]
+    with pytest.raises(ValueError, match="past the end"):
+        seq.plan_residual_norm(fake_queue, x, H=_again(_rows(fake_queue, [2], 8), starts=np.array([2 ** 32])))
+    with pytest.raises(OverflowError):
+        RaggedArray.from_buffer(np.zeros(8, np.float32), np.array([2 ** 32]), [1], [1], [1], [1])
+    with pytest.raises(OverflowError):
+        RaggedArray.from_buffer(np.zeros(8, np.float32), [2 ** 32], [1], [1], [1], [1])

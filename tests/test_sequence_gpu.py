@@ -478,6 +478,42 @@ def test_offsets_past_32_bits(queue, rng):
     close([widen(y.read_region(r * pitch, chan)) for r in range(rows)], want, mag, 60, BF16)
 
 
+def test_starts_past_32_bits(queue, rng):
+    """Items that begin 2^32 + 64 elements into their buffer, inputs and outputs, beside one at the front."""
+    chan, rows, far = 24, 5, 2 ** 32 + 64
+    starts = np.array([64, far])
+    x, y = (DeviceArray(queue, (far + 4096,), BF16) for _ in range(2))
+    ra = lambda buf, n=rows, c=chan, at=starts: CUDARaggedArray.from_buffer(queue, buf, at, [n] * 2, [c] * 2, [c] * 2, [1] * 2)
+    data = [as_dtype(normal(rng, rows, chan), BF16) for _ in starts]
+    for v, s in zip(data, starts):
+        x.write_region(s, v.ravel())
+    got = lambda: [widen(y.read_region(s, rows * chan).reshape(rows, chan)) for s in starts]
+    w = normal(rng, chan, 4)
+    seq.plan_causal_conv(queue, ra(x), vec(queue, w), ra(y))()
+    for v, g in zip(data, got()):
+        mag = S.causal_conv(widen(v), w, magnitude=True)[0]
+        close(g, S.causal_conv(widen(v), w)[0], mag, 6, BF16, "convolution")
+    seq.plan_residual_norm(queue, ra(x), H=ra(y))()
+    for v, g in zip(data, got()):
+        want = S.residual_norm(widen(v))[1]
+        close(g, want, 2 * np.abs(want), 64, BF16, "norm")
+    n, A = 8, -np.ones((chan, 8), np.float32)
+    pool = DeviceArray(queue, (far + 4096,), F32)
+    states = [normal(rng, chan, n) for _ in starts]
+    at = starts[::-1]  # (the first sequence's state far away)
+    for v, s in zip(states, at):
+        pool.write_region(s, v.ravel())
+    both = ra(pool, chan, n, at)
+    dt, short = Rows(queue, [np.full((rows, chan), 0.25)] * 2, BF16), Rows(queue, [normal(rng, rows, n)] * 2, BF16)
+    seq.plan_selective_scan(queue, ra(x), dt.ra, vec(queue, A), short.ra, short.ra, ra(y), state=both, new_state=both)()
+    for k, g in enumerate(got()):
+        args = (widen(data[k]), dt.values[k], A, short.values[k], short.values[k])
+        want, end = S.selective_scan(*args, state=states[k])
+        mag, mag_end = S.selective_scan(*args, state=states[k], magnitude=True)
+        close(g, want, mag, 100, BF16, "scan")
+        close(pool.read_region(at[k], chan * n).reshape(chan, n), end, mag_end, 100, F32, "state")
+
+
 class Block:
     """norm -> convolution -> scan -> gate, norm and residual, as one would run them."""
 
