@@ -42,6 +42,12 @@ int nb2_device_count(int* count);
 int nb2_set_device(int ordinal);
 int nb2_device_info(int ordinal, int* sm_count, int* max_threads_per_block, size_t* global_mem,
                     size_t* shared_mem_per_block_optin, int* cc_major, int* cc_minor);
+/* what memory a pointer lies in (NB2_MEM_*) and its device; changes nothing, waits for nothing */
+#define NB2_MEM_UNKNOWN 0 /* not the CUDA runtime's: ordinary host memory */
+#define NB2_MEM_HOST 1
+#define NB2_MEM_DEVICE 2
+#define NB2_MEM_MANAGED 3
+int nb2_pointer_device(const void* ptr, int* kind, int* ordinal);
 int nb2_malloc(void** dptr, size_t bytes); /* 256-byte aligned, size rounded up to 256 bytes */
 int nb2_free(void* dptr);
 int nb2_host_alloc(void** hptr, size_t bytes); /* pinned host memory */

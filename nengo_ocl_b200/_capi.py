@@ -88,6 +88,7 @@ _SIGNATURES = {
     "nb2_set_device": [c_int],
     "nb2_device_info": [c_int, POINTER(c_int), POINTER(c_int), POINTER(c_size_t), POINTER(c_size_t),
                         POINTER(c_int), POINTER(c_int)],
+    "nb2_pointer_device": [c_void_p, POINTER(c_int), POINTER(c_int)],
     "nb2_malloc": [POINTER(c_void_p), c_size_t],
     "nb2_free": [_P],
     "nb2_host_alloc": [POINTER(c_void_p), c_size_t],

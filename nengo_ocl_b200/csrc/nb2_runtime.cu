@@ -66,6 +66,18 @@ int nb2_device_info(int ordinal, int* sm_count, int* max_threads_per_block,
   return NB2_OK;
 }
 
+int nb2_pointer_device(const void* ptr, int* kind, int* ordinal) {
+  NB2_REQUIRE(kind != NULL && ordinal != NULL, "kind / ordinal");
+  cudaPointerAttributes at;
+  NB2_CUDA(cudaPointerGetAttributes(&at, ptr));
+  *kind = at.type == cudaMemoryTypeDevice    ? NB2_MEM_DEVICE
+          : at.type == cudaMemoryTypeHost    ? NB2_MEM_HOST
+          : at.type == cudaMemoryTypeManaged ? NB2_MEM_MANAGED
+                                             : NB2_MEM_UNKNOWN;
+  *ordinal = at.device;
+  return NB2_OK;
+}
+
 int nb2_malloc(void** dptr, size_t bytes) {
   NB2_REQUIRE(dptr != NULL, "dptr");
   *dptr = NULL;

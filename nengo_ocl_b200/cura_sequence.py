@@ -14,7 +14,8 @@ The same plan serves prompts and single tokens: state goes in through ``state`` 
 overlap anything else that it reads or writes; this is checked, and ``ValueError`` says what is wrong
 with an argument, ``NotImplementedError`` what the kernels do not cover.  Rows that no sequence covers
 are left as they were.  A plan owns its workspace: it can be captured and replayed, but not run on two
-streams at once.
+streams at once.  Memory has to lie on the queue's device, which is the current one while plans are built
+and run.
 """
 
 import ctypes
@@ -32,6 +33,7 @@ MAX_TAPS = 8            # NB2_CONV_MAX_TAPS
 MAX_STATES = 128        # NB2_SCAN_MAX_STATES
 KEEP_ROWS = 16          # NB2_SCAN_KEEP
 MAX_NORM_CHANNELS = 32768  # NB2_NORM_MAX_CHANNELS
+MEM_UNKNOWN, MEM_DEVICE = 0, 2  # NB2_MEM_*
 
 # Launch shapes, chosen by measurement on a B200 (148 multiprocessors).
 # Units a multiprocessor of the convolution (rows of a unit are halved, 64 to 8, until there are so many): 2 / 4 / 8 / 16
@@ -200,6 +202,18 @@ class _Arguments:
         if ary.queue.context.ordinal != self.queue.context.ordinal:
             raise ValueError("%s is on device %d, the queue on device %d"
                              % (name, ary.queue.context.ordinal, self.queue.context.ordinal))
+        self._reached(name, ary.data)
+
+    def _reached(self, name, address):
+        """The address must be memory that the queue's device reaches: a borrowed pointer may lie on another
+        one or in ordinary host memory, and what was allocated while another device was current does too."""
+        here = self.queue.context.ordinal
+        kind, ordinal = ctypes.c_int(MEM_DEVICE), ctypes.c_int(here)
+        _capi.call("nb2_pointer_device", address, ctypes.byref(kind), ctypes.byref(ordinal))
+        if kind.value == MEM_UNKNOWN:
+            raise ValueError("%s lies in host memory that the device does not reach" % name)
+        if kind.value == MEM_DEVICE and ordinal.value != here:
+            raise ValueError("%s lies on device %d, the queue on device %d" % (name, ordinal.value, here))
 
     def check_overlaps(self, in_place=()):
         """Nothing written may share memory with anything else; ``in_place``: a (read, written) pair of
@@ -253,6 +267,7 @@ class _Arguments:
             total += up(self.blocks[i][0])
             upload = total if self.blocks[i][1] is not None else upload
         memory = DeviceArray(self.queue, (total,), np.uint8)
+        self._reached("the plan's workspace (allocated on the current device)", memory.data)
         host = np.zeros(upload, np.uint8)
         for i, (nbytes, data) in enumerate(self.blocks):
             if data is not None:

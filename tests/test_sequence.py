@@ -467,3 +467,55 @@ def test_places_past_32_bits_are_not_handed_to_32_bit_tables(fake_queue):
         RaggedArray.from_buffer(np.zeros(8, np.float32), np.array([2 ** 32]), [1], [1], [1], [1])
     with pytest.raises(OverflowError):
         RaggedArray.from_buffer(np.zeros(8, np.float32), [2 ** 32], [1], [1], [1], [1])
+
+
+# ---- memory of another device --------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["conv", "scan", "norm"])
+@pytest.mark.parametrize("backward", [False, True])
+def test_memory_that_the_device_does_not_reach_is_refused(fake_queue, kind, backward):
+    """Borrowed pointers may lie anywhere, whatever their queue says; reading one there would fault."""
+    case = Case(fake_queue)
+    lib = _capi.lib()
+    stray = [0, 0, 0]  # address, kind of memory, device
+
+    def place(address, kind, ordinal):
+        if address == stray[0]:
+            kind._obj.value, ordinal._obj.value = stray[1:]
+        return 0
+
+    lib.nb2_pointer_device = place
+    build = case.backward if backward else case.forward
+    plan = case.forward(kind)
+    args = getattr(case, kind + "_grad" if backward else kind)
+    build(kind, *([plan] if backward else []))
+    for name, value in args.items():
+        if not isinstance(value, (CUDARaggedArray, DeviceArray)):
+            continue
+        stray[0] = (value.cl_buf if isinstance(value, CUDARaggedArray) else value).data
+        for stray[1], stray[2], message in ((2, 1, "on device 1"), (0, 0, "host memory")):
+            with pytest.raises(ValueError, match=message):
+                build(kind, *([plan] if backward else []))
+        for stray[1], stray[2] in ((1, 0), (3, 0), (2, 0)):  # pinned host, managed and the device's own memory
+            build(kind, *([plan] if backward else []))
+
+
+def test_a_workspace_on_another_device_is_refused(fake_queue):
+    """The current device is not the queue's while the plan is built: its table would lie on the wrong one."""
+    case = Case(fake_queue)
+    known = {v.cl_buf.data if isinstance(v, CUDARaggedArray) else v.data for kind in ("conv", "scan", "norm")
+             for v in getattr(case, kind).values() if isinstance(v, (CUDARaggedArray, DeviceArray))}
+
+    def place(address, kind, ordinal):
+        ordinal._obj.value = 0 if address in known else 1
+        return 0
+
+    _capi.lib().nb2_pointer_device = place
+    for kind in ("conv", "scan", "norm"):
+        with pytest.raises(ValueError, match="workspace.*device 1"):
+            case.forward(kind)
+
+
+def test_memory_kinds_agree_with_the_header():
+    c = _capi.header_constants("NB2_MEM_")
+    assert (seq.MEM_UNKNOWN, seq.MEM_DEVICE) == (c["NB2_MEM_UNKNOWN"], c["NB2_MEM_DEVICE"])
+    assert _capi.lib().nb2_pointer_device(None, None, None) == -2

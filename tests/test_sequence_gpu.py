@@ -632,6 +632,24 @@ def test_torch_memory_is_used_in_place(ctx, rng):
     close(h.double().cpu().numpy(), want, 2 * np.abs(want), 64, BF16)
 
 
+def test_host_memory_is_refused_unless_the_device_reaches_it(ctx, queue, rng):
+    torch = pytest.importorskip("torch")
+    x = Rows(queue, [normal(rng, 6, 40)], F32)
+    host = np.zeros(240, np.float32)
+    ra = lambda address, base: CUDARaggedArray.from_buffer(queue, DeviceArray(queue, (240,), F32, data=address, base=base),
+                                                           [0], [6], [40], [40], [1])
+    with pytest.raises(ValueError, match="host memory"):  # (refused when the plan is built: nothing is launched)
+        seq.plan_residual_norm(queue, x.ra, H=ra(host.ctypes.data, host))
+    pinned = torch.zeros(240).pin_memory()
+    seq.plan_residual_norm(queue, x.ra, H=ra(pinned.data_ptr(), pinned))()
+    want = S.residual_norm(x.values[0])[1]
+    close(pinned.numpy().reshape(6, 40), want, 2 * np.abs(want), 64, F32)
+    with torch.cuda.device(0):
+        mine = torch.zeros(240, device="cuda")
+    seq.plan_residual_norm(queue, x.ra, H=ra(mine.data_ptr(), mine))()
+    assert np.array_equal(mine.cpu().numpy(), pinned.numpy())
+
+
 def test_the_plans_device_must_be_current(queue, rng):
     """A launch whose plan names another device than the current one is refused, not run."""
     from nengo_ocl_b200 import _capi
