@@ -24,7 +24,7 @@ import numpy as np
 
 from nengo_ocl_b200.raggedarray import _DTYPES, RaggedArray
 from nengo_ocl_b200.runtime import DeviceArray, to_device
-from nengo_ocl_b200.utils import as_dtype, bfloat16, equal_strides, is_iterable
+from nengo_ocl_b200.utils import as_dtype, bfloat16, equal_strides, is_bfloat16, is_iterable
 
 
 def to_host(queue, darray, dtype, start, shape, elemstrides):
@@ -208,8 +208,8 @@ class CUDARaggedArray:
         start = int(self.index64("starts")[item])
         if m * n == 0:
             return
-        if self.dtype == bfloat16:
-            new_value = as_dtype(new_value, bfloat16)
+        if self.dtype == bfloat16 or is_bfloat16(new_value):
+            new_value = as_dtype(new_value, self.dtype)
             new_value = new_value.reshape(m, n) if new_value.size == m * n else np.broadcast_to(new_value, (m, n))
         if (sm, sn) in [(1, m), (n, 1)] or equal_strides((sm, sn), (n, 1), (m, n)):
             # contiguous: one write

@@ -67,7 +67,7 @@ class RaggedArray:
 
         buf = np.zeros(starts[-1] + sizes[-1], dtype=dtype)
         for a, s in zip(arrays, starts):
-            buf[s : s + a.size] = as_dtype(a, dtype).ravel() if dtype == bfloat16 else a.ravel()
+            buf[s : s + a.size] = as_dtype(a, dtype).ravel()
         self.buf = buf
         self.names = names
 
@@ -210,6 +210,8 @@ class RaggedArray:
             item = int(item)
         except TypeError as e:
             raise NotImplementedError("`item` must be castable to int") from e
+        if bfloat16 in (self.dtype, getattr(value, "dtype", None)):
+            value = as_dtype(value, self.dtype)
         self[item][...] = value
 
     def add_views(self, starts, shape0s, shape1s, stride0s, stride1s, names=None):

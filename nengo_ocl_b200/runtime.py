@@ -13,7 +13,7 @@ import weakref
 import numpy as np
 
 from nengo_ocl_b200 import _capi
-from nengo_ocl_b200.utils import bfloat16
+from nengo_ocl_b200.utils import as_dtype, bfloat16, from_bfloat16, is_bfloat16
 
 
 class Device:
@@ -161,18 +161,20 @@ class DeviceArray:
         return out
 
     def set(self, array):
-        array = np.ascontiguousarray(array, dtype=self.dtype)
+        array = np.ascontiguousarray(as_dtype(array, self.dtype))
         assert array.size == self.size
         if self.nbytes:
             _capi.call("nb2_memcpy_h2d", self.ptr, array.ctypes.data_as(ctypes.c_void_p), self.nbytes,
                        self.queue.stream, 1)
 
     def fill(self, value):
+        if is_bfloat16(value):
+            value = from_bfloat16(value)
         if np.all(np.asarray(value) == 0):
             _capi.call("nb2_memset", self.ptr, 0, self.nbytes, self.queue.stream)
             self.queue.finish()
         else:
-            self.set(np.full(self.shape, value, dtype=self.dtype))
+            self.set(np.broadcast_to(as_dtype(value, self.dtype), self.shape))
 
     def read_region(self, elem_start, n_elems):
         """Blocking copy of ``n_elems`` elements starting at ``elem_start``."""
@@ -185,7 +187,7 @@ class DeviceArray:
         return out
 
     def write_region(self, elem_start, array):
-        array = np.ascontiguousarray(array, dtype=self.dtype)
+        array = np.ascontiguousarray(as_dtype(array, self.dtype))
         if array.size:
             isz = self.dtype.itemsize
             _capi.call("nb2_memcpy_h2d", ctypes.c_void_p(self.data + int(elem_start) * isz),

@@ -39,6 +39,10 @@ def as_dtype(array, dtype):
     return (from_bfloat16(array) if array.dtype == bfloat16 else array).astype(dtype, copy=False)
 
 
+def is_bfloat16(value):
+    return getattr(value, "dtype", None) == bfloat16
+
+
 def is_iterable(obj):
     """True for lists/tuples/ranges and ndarrays with ndim > 0 (not scalars)."""
     if isinstance(obj, np.ndarray):

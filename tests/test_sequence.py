@@ -106,6 +106,42 @@ def test_ragged_arrays_of_16_bit_types(rng, fake_queue):
         RaggedArray(values, dtype=np.float64)
 
 
+def test_values_cross_between_bfloat16_and_other_types(rng, fake_queue):
+    """Host values go into an array of another type as values, not as the integers that bfloat16 is stored as."""
+    v = rng.normal(size=(3, 4)).astype(np.float32)
+    short = to_bfloat16(v)
+    into = {np.dtype(np.float32): from_bfloat16(short), np.dtype(np.float16): from_bfloat16(short).astype(np.float16),
+            bfloat16: short}
+    for dtype, want in into.items():
+        two = to_bfloat16(np.float32(2)) if dtype == bfloat16 else dtype.type(2)
+        for source in (v, v.astype(np.float64)) if dtype == bfloat16 else (short,):
+            d = DeviceArray(fake_queue, (3, 4), dtype)
+            d.set(source)
+            assert np.array_equal(d.get(), want)
+            d.fill(2.0)
+            assert (d.get() == two).all()
+            d.write_region(4, source[0])
+            assert np.array_equal(d.get()[1], want[0]) and (d.get()[0] == two).all()
+            ra = RaggedArray([source, source[:2]], dtype=dtype)
+            assert np.array_equal(ra[0], want) and np.array_equal(ra[1], want[:2])
+            ra[1] = 2.0
+            assert (ra[1] == two).all()
+            ra[1] = source[1:]
+            assert np.array_equal(ra[1], want[1:])
+            clra = CUDARaggedArray(fake_queue, ra)
+            clra[1] = 2.0
+            assert (clra[1] == two).all()
+            clra[1] = source[:2]
+            assert np.array_equal(clra[1], want[:2])
+            turned = CUDARaggedArray.from_buffer(fake_queue, clra.cl_buf, [0], [2], [3], [4], [1])
+            turned[0] = source[:2, :3]
+            assert np.array_equal(turned[0], want[:2, :3])
+        d.fill(to_bfloat16(np.float32(2)))
+        assert (d.get() == two).all()
+        d.fill(to_bfloat16(np.float32(0)))
+        assert not d.get().view(np.uint8).any()
+
+
 # ---- which rows share memory -------------------------------------------------------------------
 def test_shared_bytes_against_enumeration(rng):
     def cells(low, rows, pitch, width):
