@@ -64,9 +64,11 @@ __global__ void __launch_bounds__(NormThreads<NV>::kMost, NV == 1 ? 2 : 1) nb2_r
       for (int e = 0; e < V; ++e) {
         float v = u[i][e] * inv;
         if constexpr (GATE == kGateLast) v *= gv[e] * nb2_sigmoid(gv[e]);
-        u[i][e] = fmaf(w[e], v, rv[e]);  // (zeros past the row's end)
+        u[i][e] = fmaf(w[e], v, rv[e]);
         ss[i] = fmaf(u[i][e], u[i][e], ss[i]);
       }
+      // (past the row's end: 0 times an infinite 1 / sqrt(0 + eps), weight or scale, left out of the sum)
+      if (tid + i * step >= vecs) ss[i] = 0.0f;
       if (y && tid + i * step < vecs) {
         o.put(u[i]);
         o.store(y + i * step * V);

@@ -99,14 +99,17 @@ __global__ void __launch_bounds__(NormThreads<NV>::kMost, 1) nb2_residual_norm_g
         if constexpr (GATE == kGateLast) in.get(1, i, t, gv);
         in.get(2, i, t, rv);
         in.get(4, i, t, dh);
+        float mine[2] = {ss[0], ss[1]};
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           float v = u[i][e];
           if constexpr (GATE == kGateLast) v *= gv[e] * s[i][e];
-          r[i][e] = fmaf(w[e], v, rv[e]);  // (zeros past the row's end)
-          ss[0] = fmaf(r[i][e], r[i][e], ss[0]);
-          ss[1] = fmaf(dh[e] * wn[e], r[i][e], ss[1]);
+          r[i][e] = fmaf(w[e], v, rv[e]);
+          mine[0] = fmaf(r[i][e], r[i][e], mine[0]);
+          mine[1] = fmaf(dh[e] * wn[e], r[i][e], mine[1]);
         }
+        // (past the row's end: 0 times an infinite 1 / sqrt(0 + eps), weight or scale, left out of the sums)
+        if (tid + i * step < vecs) ss[0] = mine[0], ss[1] = mine[1];
       }
       // both sums with one barrier
 #pragma unroll
@@ -157,6 +160,7 @@ __global__ void __launch_bounds__(NormThreads<NV>::kMost, 1) nb2_residual_norm_g
         r[i][e] = dr[e] * w[e];  // q (without the late gate) from here on
         part[i] = fmaf(r[i][e], hat, part[i]);
       }
+      if (tid + i * step >= vecs) part[i] = 0.0f;
       if (dresidual && tid + i * step < vecs) {
         o.put(dr);
         o.store(dresidual + i * step * V);

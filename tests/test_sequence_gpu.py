@@ -440,6 +440,30 @@ def test_residual_norm(queue, rng, dtype, lengths, chan, groups, pad, lead, gate
             close(dev_.get(), sums[name][0], sums[name][1], 2 * chain + sum(lengths), F32, name)
 
 
+@DTYPES
+@pytest.mark.parametrize("eps", [0.0, 1e-42, 0.1])
+@pytest.mark.parametrize("gate_first", [True, False])
+@pytest.mark.parametrize("chan,groups", [(1000, 5), (1000, 1), (80, 5), (160, 5), (40, 1), (35, 7), (35, 1), (1280, 5),
+                                         (8200, 5), (8200, 1)])
+def test_norm_eps(queue, rng, monkeypatch, dtype, eps, gate_first, chan, groups):
+    """Other eps than the usual one, zero among them (1e-42 is below float32's normal numbers), with rows that
+    do not fill their block of threads: the threads past the end add nothing."""
+    for f in (seq.plan_residual_norm, S.residual_norm, S.residual_norm_grad):
+        monkeypatch.setattr(f, "__defaults__", tuple(eps if d == 1e-5 else d for d in f.__defaults__))
+    test_residual_norm(queue, rng, dtype, [3, 0, 2], chan, groups, 0, 0, True, gate_first, True, True, True, True, True, True)
+
+
+def test_norm_infinite_weight_stays_in_its_channel(queue, rng):
+    """The last channel's infinite weight: the row's norm is infinite, so every other h is zero, none is NaN."""
+    chan = 1000
+    x, h = Rows(queue, [normal(rng, 2, chan)], F32), Rows(queue, [np.zeros((2, chan))], F32, empty=True)
+    w = np.ones(chan, np.float32)
+    w[-1] = np.inf
+    seq.plan_residual_norm(queue, x.ra, H=h.ra, weight=vec(queue, w), groups=5)()
+    got = h.get()[0]
+    assert (got[:, :-1] == 0).all() and np.isnan(got[:, -1]).all()
+
+
 def test_norm_of_zero_rows_and_infinities(queue, rng):
     x = np.zeros((3, 40), np.float32)
     x[1, 3] = np.inf
