@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(256) nb2_scan_join_kernel(const ScanJoin a) {
   if (k >= a.n_seq) return;
   const int64_t cn = i - k * a.per_seq, c = cn / a.n_states, len = a.table[k];
   const int64_t u0 = a.table[a.first_unit_field * a.n_seq + k], units = max((len + a.unit_rows - 1) / a.unit_rows, (int64_t)1);
-  const float A2 = a.A[cn] * LOG2E;
+  const float A2 = scan_rate(a.A[cn]);
   float h = 0.0f;
   if (a.from) {
     const ScanPlace p = scan_place(a.table, a.n_seq, a.from_array, k);
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 8) nb2_selective_scan_token_kern
     ch[u] = group * per + min(at, per - 1);
     scan_load4(a.A + (int64_t)ch[u] * n, n0, n, n % 4 == 0 && a.a_vec, A2[u]);
 #pragma unroll
-    for (int m = 0; m < 4; ++m) A2[u][m] *= LOG2E;
+    for (int m = 0; m < 4; ++m) A2[u][m] = scan_rate(A2[u][m]);
     D[u] = a.D ? a.D[ch[u]] : 0.0f;
     bias[u] = a.dt_bias ? a.dt_bias[ch[u]] : 0.0f;
   }

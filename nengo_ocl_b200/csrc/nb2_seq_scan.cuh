@@ -291,16 +291,19 @@ __device__ __forceinline__ void scan_clear_weights(Stage* stages, int count) {
   for (int i = threadIdx.x; i < count * kEach; i += SCAN_THREADS) (&stages[i / kEach].bc[0][0][0])[i % kEach] = 0.0f;
 }
 
-// A[c][n0 ..] log2(e), two states to a register pair.  Held finite: a row past a sequence's end counts as a
-// step of zero, which has to leave the state as it is (0 * inf would not).
+// A log2(e), held finite: a step of zero (a masked row, or one past a sequence's end) has to leave the state as it
+// is, which 0 * inf would not.
+__device__ __forceinline__ float scan_rate(float A) {
+  const float r = A * LOG2E;
+  return r > 3e38f ? 3e38f : r < -3e38f ? -3e38f : r;
+}
+
+// A[c][n0 ..] log2(e), two states to a register pair
 __device__ __forceinline__ void scan_rates(const float* A, int n0, int n, f32x2 (&A2)[2]) {
   float v[4];
   scan_load4(A, n0, n, 0, v);
 #pragma unroll
-  for (int m = 0; m < 4; ++m) {
-    const float r = v[m] * LOG2E;
-    v[m] = r > 3e38f ? 3e38f : r < -3e38f ? -3e38f : r;
-  }
+  for (int m = 0; m < 4; ++m) v[m] = scan_rate(v[m]);
   A2[0] = pack2(v[0], v[1]);
   A2[1] = pack2(v[2], v[3]);
 }

@@ -343,6 +343,45 @@ def test_scan_forgets_at_infinite_decay(queue, rng):
         close(end, own[-1], np.abs(own[-1]), 4, F32, "new_state")
 
 
+@pytest.mark.parametrize("lengths,split", [([210, 0, 33], True), ([1, 2, 0, 1], False), ([40, 90], False)], ids=str)
+def test_zero_steps_at_infinite_decay(queue, rng, lengths, split):
+    """A = -inf and masked rows (a step of zero) among others: such a row leaves the state as it is, wherever the
+    sequence is split and whichever kernel takes it.  The oracle's A is -1e30, which decays as completely."""
+    s = Scan(queue, rng, lengths, 8, 4, 1, F32, bias=False, softplus=False)
+    for k, n in enumerate(lengths):
+        s.dt.values[k][(2 * n) // 10:(8 * n + 9) // 10] = 0
+    s.dt = Rows(queue, s.dt.values, F32, columns=8)
+    s.A[:] = -np.inf
+    s.params["A"] = vec(queue, s.A)
+    plan = s.plan()
+    assert (plan.full_args[0].n_units > len(lengths)) == split and bool(plan.full_args[0].tokens) == (max(lengths) < 3)
+    dy = Rows(queue, [normal(rng, n, 8) for n in lengths], F32, columns=8)
+    outs = {name: Rows(queue, r.values, F32, empty=True, columns=r.place[0][2])
+            for name, r in (("dx", s.x), ("ddt", s.dt), ("dB", s.B), ("dC", s.C))}
+    dstate, dnew = Rows(queue, s.state.values, F32, empty=True), Rows(queue, [normal(rng, 8, 4) for _ in lengths], F32)
+    dA = vec(queue, np.full((8, 4), 9.0))
+    plan()
+    y, new = s.y.get(), s.new.get()
+    fwd = s.plan(keep=True)
+    bwd = seq.plan_selective_scan_grad(queue, fwd, dy.ra, outs["dx"].ra, outs["ddt"].ra, dA, outs["dB"].ra, outs["dC"].ra,
+                                       dstate=dstate.ra, dnew_state=dnew.ra)
+    assert (bwd.full_args[0].n_units > len(lengths)) == split
+    fwd()
+    bwd()
+    assert (dA.get() == 0).all()
+    for k in range(len(lengths)):
+        args = dict(s.of(k), A=np.full((8, 4), -1e30))
+        want, size = S.selective_scan(**args), S.selective_scan(**args, magnitude=True)
+        for got in ((y[k], new[k]), (s.y.get()[k], s.new.get()[k])):
+            for g, w, m, what in zip(got, want, size, ("y", "new_state")):
+                close(g, w, m, lengths[k] * 6 + 200, F32, what)
+        grads = dict(args, dy=dy.values[k], dnew_state=dnew.values[k])
+        want, size = S.selective_scan_grad(**grads), S.selective_scan_grad(**grads, magnitude=True)
+        for name, r in dict(outs, dstate=dstate).items():
+            if name != "ddt":  # (q A of a state that stays: infinite)
+                close(r.get()[k], want[name], size[name], 2 * (lengths[k] * 6 + 300), F32, name)
+
+
 # ---- norms ---------------------------------------------------------------------------------------
 NORMS = [  # chan, groups, pad, lead, gate, gate_first, residual, weight, scale, norm_weight, Y, H
     (1, 1, 0, 0, True, True, True, True, True, True, True, True),
