@@ -254,7 +254,10 @@ __global__ void __launch_bounds__(256) nb2_scan_join_kernel(const ScanJoin a) {
     for (int q = 0; q < kAhead; ++q) {
       if (u + q >= units) break;
       ends[(u + q) * step * a.per_seq] = h;
-      h = fmaf(scan_exp2(s[q] * A2), h, e[q]);
+      // row by row a growing state reaches infinity only where it is: nothing comes of zero, and half the exponent at
+      // a time a small start does not meet a factor past the range
+      const float half = scan_exp2(0.5f * (s[q] * A2));
+      h = h == 0.0f ? e[q] : fmaf(half, half * h, e[q]);
     }
   }
 }

@@ -382,6 +382,37 @@ def test_zero_steps_at_infinite_decay(queue, rng, lengths, split):
                 close(r.get()[k], want[name], size[name], 2 * (lengths[k] * 6 + 300), F32, name)
 
 
+def test_growing_states_over_split_sequences(queue, rng):
+    """A > 0 (and steps of both signs): over a unit of 32 rows the growth passes float32's range, the states do
+    not.  A zero state stays zero, a small one grows to what it is row by row."""
+    lengths = [224, 224]
+    s = Scan(queue, rng, lengths, 8, 4, 1, F32, bias=False, softplus=False, D=False, gate=False)
+    sign = np.where(np.arange(224) // 32 % 2, -1.0, 1.0)[:, None]
+    s.dt = Rows(queue, [np.broadcast_to(sign, (224, 8))] * 2, F32)
+    x = np.zeros((224, 8), np.float32)
+    x[200:] = normal(rng, 24, 8) * 1e-20  # (rows that grow, for less than a unit)
+    s.x = Rows(queue, [x, x], F32)
+    s.A = np.full((8, 4), 4.0, np.float32)  # 32 rows: e^128
+    s.params["A"] = vec(queue, s.A)
+    state = np.full((8, 4), 1e-30, np.float32)
+    s.state = Rows(queue, [np.zeros((8, 4)), state], F32)
+    dy = Rows(queue, [np.where(np.arange(224)[:, None] < 20, 1e-20, 0) * normal(rng, 224, 8) for _ in lengths], F32)
+    outs = [Rows(queue, r.values, F32, empty=True) for r in (s.x, s.dt, s.B, s.C)]
+    dnew = Rows(queue, [np.zeros((8, 4)), state], F32)
+    dstate, dA = Rows(queue, [state] * 2, F32, empty=True), vec(queue, np.zeros((8, 4)))
+    fwd = s.plan(keep=True)
+    bwd = seq.plan_selective_scan_grad(queue, fwd, dy.ra, outs[0].ra, outs[1].ra, dA, outs[2].ra, outs[3].ra,
+                                       dstate=dstate.ra, dnew_state=dnew.ra)
+    assert fwd.full_args[0].unit_rows == bwd.full_args[0].unit_rows == 32
+    fwd()
+    bwd()
+    s.check()
+    for k in range(2):
+        args = dict(s.of(k), dy=dy.values[k], dnew_state=dnew.values[k])
+        want, size = S.selective_scan_grad(**args), S.selective_scan_grad(**args, magnitude=True)
+        close(dstate.get()[k], want["dstate"], size["dstate"], 2 * s.chain(k, 300), F32, "dstate")
+
+
 # ---- norms ---------------------------------------------------------------------------------------
 NORMS = [  # chan, groups, pad, lead, gate, gate_first, residual, weight, scale, norm_weight, Y, H
     (1, 1, 0, 0, True, True, True, True, True, True, True, True),
