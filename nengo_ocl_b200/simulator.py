@@ -1089,7 +1089,8 @@ class Simulator:
     def _plan_sequence_ops(self, ops, shared, same, rows, make):
         plans = []
         key = lambda op: (tuple(getattr(op, n) if not isinstance(getattr(op, n), Signal) else id(getattr(op, n))
-                                for n in shared + same), op.x.size, tuple(getattr(op, n) is None for n in rows))
+                                for n in shared + same),
+                          tuple(None if getattr(op, n) is None else getattr(op, n).size for n in rows))
         for _, group in groupby(ops, key):
             args = {n: self._row_items([getattr(op, n) for op in group]) for n in rows}
             args.update({n: self._parameter(getattr(group[0], n)) if isinstance(getattr(group[0], n), (Signal, type(None)))

@@ -430,6 +430,40 @@ def test_model_operators_are_planned_once_per_parameter_set(monkeypatch):
     sim.close()
 
 
+def two_widths_model(channels=8, n_states=4):
+    """Scans that share A, D and dt_bias, with B and C for one group of channels and for two."""
+    from nengo_ocl_b200 import model as m
+
+    rng = np.random.RandomState(3)
+    mdl = m.Model(dt=0.001)
+    const = lambda name, v: m.Signal(v, name=name, readonly=True)
+    A, D = const("A", -rng.uniform(0.5, 4, size=(channels, n_states))), const("D", rng.normal(size=channels))
+    bias = const("dt_bias", rng.uniform(-2, 0, size=channels))
+    outs = []
+    for k, groups in enumerate((1, 2, 1)):
+        row = lambda name, n: m.Signal(rng.normal(size=n), name="%s%d" % (name, k))
+        x, dt, B, C = row("x", channels), row("dt", channels), row("B", groups * n_states), row("C", groups * n_states)
+        y, state = m.Signal(np.zeros(channels), name="y%d" % k), m.Signal(np.zeros((channels, n_states)), name="s%d" % k)
+        mdl.add_op(m.SimSelectiveScan(x, dt, A, B, C, y, state, D=D, dt_bias=bias))
+        outs += [y, state]
+    mdl.info = dict(outs=outs)
+    return mdl
+
+
+def test_model_scans_of_other_widths_are_planned_apart(monkeypatch):
+    from nengo_ocl_b200 import runtime
+    from nengo_ocl_b200 import simulator as sim_mod
+
+    fake_library.install(monkeypatch)
+    monkeypatch.setattr(sim_mod.Simulator, "some_context", None)
+    monkeypatch.setattr(runtime, "_default_context", None, raising=False)
+    sim = sim_mod.Simulator(None, model=two_widths_model())
+    plans = [p for p in sim._plans if p.name == "cura_selective_scan"]
+    assert sorted(len(p.sequence_args["X"]) for p in plans) == [1, 2]
+    assert sorted(p.sequence_args["groups"] for p in plans) == [1, 2]
+    sim.close()
+
+
 def test_oracle_steps_equal_whole_sequences():
     """The operator-list interpreter's step-by-step block against one pass over all rows."""
     from nengo_ocl_b200 import synth

@@ -784,3 +784,18 @@ def test_simulated_block_matches_the_oracle(ctx):
             assert first is None or all(np.array_equal(a, b) for a, b in zip(first, data))
             first = data
             sim.reset()
+
+
+def test_simulated_scans_of_other_widths(ctx):
+    from nengo_ocl_b200.simulator import Simulator
+    from oracle.simulator import OracleSimulator
+    from test_sequence import two_widths_model
+
+    mdl = two_widths_model()
+    ora = OracleSimulator(mdl)
+    ora.run_steps(9)
+    with Simulator(None, model=mdl, context=ctx) as sim:
+        sim.run_steps(9)
+        for s in mdl.info["outs"]:
+            # (nine rows of a decaying state of order one: 9 (6 + 30 * 4 * 2) + 200 half steps)
+            assert np.allclose(sim.signals[s].ravel(), ora[s].ravel(), rtol=2e-4, atol=2e-4)
