@@ -120,6 +120,8 @@ class _Arguments:
             raise NotImplementedError("sequences of type %s" % self.dtype)
         self.lengths = X.shape0s.astype(np.int64)
         self.channels = int(X.shape1s[0])
+        if self.channels < 1:
+            raise ValueError("%s has no channels" % what)
         self.memory = []
         self.fields = []
         self.kept = []
@@ -438,7 +440,7 @@ def plan_selective_scan(queue, X, dt, A, B, C, Y, D=None, Z=None, dt_bias=None, 
         raise ValueError("B must be a CUDARaggedArray with an item per sequence")
     width = int(B.shape1s[0])
     groups = width // n
-    if width % n or a.channels % groups:
+    if groups < 1 or width % n or a.channels % groups:
         raise ValueError("B has %d columns: a multiple of the %d states that divides the channels is expected"
                          % (width, n))
     per = np.full(len(a.lengths), a.channels, np.int64)

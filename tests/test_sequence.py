@@ -302,6 +302,17 @@ def test_sizes_out_of_range_are_refused(fake_queue):
         wide.forward("norm")
 
 
+def test_arrays_without_columns_are_refused(fake_queue):
+    q = fake_queue
+    case = Case(q)
+    with pytest.raises(ValueError, match="multiple"):
+        case.forward("scan", B=_rows(q, [5, 0, 3], 0), C=_rows(q, [5, 0, 3], 0))
+    empty = Case(q, chan=0)
+    for kind in ("conv", "scan", "norm"):
+        with pytest.raises(ValueError, match="no channels"):
+            empty.forward(kind)
+
+
 def test_overlapping_outputs_are_refused(fake_queue):
     case = Case(fake_queue)
     for kind, outs in (("conv", ["Y", "new_state"]), ("scan", ["Y", "new_state"]), ("norm", ["Y", "H"])):
