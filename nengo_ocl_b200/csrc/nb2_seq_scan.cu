@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, VEC ? 6 : 4) nb2_selective_scan_
     weights.load((const T*)b.p + from * b.stride, b.stride, (const T*)c.p + from * c.stride, c.stride, n, rows);
   };
   auto arrive = [&](Stage& st) {
-    weights.store(st.bc, n);
+    weights.store(st.bc);
 #pragma unroll
     for (int i = 0; i < NA; ++i)
       if (i != kZ || gate) copy[i].store(st.in[i]);

@@ -165,14 +165,15 @@ struct ScanArray {
 };
 
 // What a block stages in shared memory: R rows of its channels of NA arrays in their own type, and the
-// rows' weights B, C in float32 (converted once for all its channels), padded with zeros to 4 S states.
-template <typename T, int S, int P, int R, int NA>
+// rows' weights B, C in float32 (converted once for all its channels), padded with zeros to 4 S states and, for
+// sums over channels (ZEROS), four zeros more: those of a lane without a channel, whatever B and C hold.
+template <typename T, int S, int P, int R, int NA, bool ZEROS = false>
 struct ScanStage {
   static constexpr int kChannels = SCAN_THREADS / S * P, kRows = R;
   // rows that a warp's lanes read at the same time start in different banks
   static constexpr int kPad = (P * (int)sizeof(T) < 4 ? P * (int)sizeof(T) : 4) * 32 / S;
   static constexpr int kPitch = (kChannels * (int)sizeof(T) + kPad + 15) / 16 * 16 / (int)sizeof(T);
-  static constexpr int kStates = 4 * S;
+  static constexpr int kStates = 4 * S + (ZEROS ? 4 : 0);
   static constexpr int kBytes = kChannels * (int)sizeof(T) < 16 ? kChannels * (int)sizeof(T) : 16;
   alignas(16) T in[NA][R][kPitch];
   alignas(16) float bc[R][2][kStates];
@@ -276,12 +277,13 @@ struct ScanWeights {
       if (to[i] >= 0 && r < rows) v[i].load((to[i] & (4 * S) ? C + r * cs : B + r * bs) + m);
     }
   }
-  __device__ __forceinline__ void store(float (&bc)[R][2][4 * S], int n) const {
+  template <int PITCH>
+  __device__ __forceinline__ void store(float (&bc)[R][2][PITCH]) const {
 #pragma unroll
     for (int i = 0; i < kCount; ++i)
       if (to[i] >= 0)
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) (&bc[0][0][0])[to[i] + e] = v[i][e];
+        for (int e = 0; e < kPer; ++e) (&bc[0][0][0])[to[i] / (4 * S) * (PITCH - 4 * S) + to[i] + e] = v[i][e];
   }
 };
 

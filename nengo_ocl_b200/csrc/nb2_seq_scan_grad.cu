@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) nb2_scan_grad_ends_kernel(const 
     weights.load(B + from * pb.stride, pb.stride, C + from * pc.stride, pc.stride, n, rows);
   };
   auto arrive = [&](Stage& st) {
-    weights.store(st.bc, n);
+    weights.store(st.bc);
 #pragma unroll
     for (int i = 0; i < NA; ++i) copy[i].store(st.in[i]);
   };
@@ -152,7 +152,7 @@ template <typename T, int S, bool VEC>
 __global__ void __launch_bounds__(SCAN_THREADS, S < 16 ? 4 : 3) nb2_selective_scan_grad_kernel(const nb2_selective_scan_grad_args a) {
   constexpr int R = NB2_SCAN_KEEP, RB = S < 4 ? S : 4;
   constexpr int NA = 4;
-  using Stage = ScanStage<T, S, 1, R, NA>;
+  using Stage = ScanStage<T, S, 1, R, NA, true>;
   using Sum = ScanChannelSum<S>;
   extern __shared__ __align__(16) char smem_raw[];
   Stage* stages = reinterpret_cast<Stage*>(smem_raw);
@@ -194,7 +194,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 ? 4 : 3) nb2_selective_sc
   const float D = a.D ? a.D[c] : 0.0f, bias = a.dt_bias ? a.dt_bias[c] : 0.0f;
   const int j = l.j % RB, mine = l.in_block;
   const bool stores = l.valid(0) && l.j < RB;
-  float dD = 0.0f, dbias = 0.0f, h0[4];
+  // A lane without a channel adds nothing to dB and dC: steps, gradients, weights and states of zero.
+  const int bc0 = l.valid(0) ? l.n0 : 4 * S;
+  float dD = 0.0f, dbias = 0.0f, h0[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   scan_clear_weights(stages, 2);
   __syncthreads();
   ScanWeights<VEC, T, S, R> weights(n);
@@ -208,10 +210,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 ? 4 : 3) nb2_selective_sc
       }
     const ScanArray b = sm.arrays[kB], c = sm.arrays[kC];
     weights.load((const T*)b.p + from * b.stride, b.stride, (const T*)c.p + from * c.stride, c.stride, n, rows);
-    scan_load4(keep + from / R * a.channels * n, l.n0, n, n % 4 == 0, h0);
+    if (l.valid(0)) scan_load4(keep + from / R * a.channels * n, l.n0, n, n % 4 == 0, h0);
   };
   auto arrive = [&](Stage& st) {
-    weights.store(st.bc, n);
+    weights.store(st.bc);
 #pragma unroll
     for (int i = 0; i < NA; ++i) copy[i].store(st.in[i]);
   };
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 ? 4 : 3) nb2_selective_sc
             const float zv = nb2_to_float(st.in[3][r][mine]);
             dp *= zv * nb2_sigmoid(zv);
           }
-          if (r >= rows || !l.valid(0)) {  // (a lane without a channel adds nothing to dB, dC)
+          if (r >= rows || !l.valid(0)) {
             o = make_float2(0.0f, 0.0f);
             dp = 0.0f;
           }
@@ -268,7 +270,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 ? 4 : 3) nb2_selective_sc
       for (int r = 0; r < H; ++r) {
         f32x2 s2[1], x2[1];
         sm.ready.get(r, mine, s2, x2);
-        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&st.bc[r][0][l.n0]);
+        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&st.bc[r][0][bc0]);
         mid[0] = fma2(exp2x2(mul2(s2[0], A2[0])), mid[0], mul2(x2[0], b.x));
         mid[1] = fma2(exp2x2(mul2(s2[0], A2[1])), mid[1], mul2(x2[0], b.y));
       }
@@ -280,7 +282,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 ? 4 : 3) nb2_selective_sc
       for (int i = 0; i < H; ++i) {
         f32x2 s2[1], x2[1];
         sm.ready.get(rb + i, mine, s2, x2);
-        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&st.bc[rb + i][0][l.n0]);
+        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&st.bc[rb + i][0][bc0]);
         dec[i][0] = exp2x2(mul2(s2[0], A2[0]));
         dec[i][1] = exp2x2(mul2(s2[0], A2[1]));
         h[i][0] = fma2(dec[i][0], i ? h[i ? i - 1 : 0][0] : from[0], mul2(x2[0], b.x));
@@ -296,8 +298,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 ? 4 : 3) nb2_selective_sc
           sm.ready.get(r, mine, s2, x2);
           const float dp = sm.dp[r][mine];
           const f32x2 d2 = pack2(dp, dp);
-          const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&st.bc[r][0][l.n0]);
-          const ulonglong2 cw = *reinterpret_cast<const ulonglong2*>(&st.bc[r][1][l.n0]);
+          const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&st.bc[r][0][bc0]);
+          const ulonglong2 cw = *reinterpret_cast<const ulonglong2*>(&st.bc[r][1][bc0]);
           const f32x2 h0 = h[q + i][0], h1 = h[q + i][1];
           const f32x2 g0 = fma2(cw.x, d2, carry[0]), g1 = fma2(cw.y, d2, carry[1]);
           carry[0] = mul2(g0, dec[q + i][0]);
@@ -456,7 +458,7 @@ static cudaError_t scan_grad_units(cudaStream_t s, const nb2_selective_scan_grad
     SCAN_TRY(nb2_launch(nb2_scan_grad_ends_kernel<T, S, VEC>, grid, block, smem, s, a));
     SCAN_TRY(nb2_scan_join(s, ScanJoin{a.table, a.n_seq, a.n_states, a.unit_rows, 1, a.channels, 0, 29, a.A, a.dnew_state, 12, a.ends, a.sums}));
   }
-  const size_t smem = 2 * sizeof(ScanStage<T, S, 1, R, 4>) + sizeof(ScanGradSmem<S>);
+  const size_t smem = 2 * sizeof(ScanStage<T, S, 1, R, 4, true>) + sizeof(ScanGradSmem<S>);
   SCAN_TRY(scan_allow_smem(nb2_selective_scan_grad_kernel<T, S, VEC>, smem));
   return nb2_launch(nb2_selective_scan_grad_kernel<T, S, VEC>, grid, block, smem, s, a);
 }

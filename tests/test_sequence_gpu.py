@@ -413,6 +413,37 @@ def test_growing_states_over_split_sequences(queue, rng):
         close(dstate.get()[k], want["dstate"], size["dstate"], 2 * s.chain(k, 300), F32, "dstate")
 
 
+@pytest.mark.parametrize("chan,groups,n", [(40, 1, 16), (66, 2, 12), (9, 1, 64), (130, 1, 4), (3, 3, 128)])
+@pytest.mark.parametrize("which", ["B", "C"])
+def test_infinite_weights_of_a_partial_tile(queue, rng, which, chan, groups, n):
+    """One infinite value of B (or C): with positive inputs dC of its row and the later ones (dB of its row and
+    the earlier ones) is infinite in that state, nothing is NaN, and the rest is what it is without it.  The blocks'
+    channels do not fill them, and what the idle lanes hold must not get into the sums over channels."""
+    rows, at, state = 21, 9, n // 2
+    s = Scan(queue, rng, [rows], chan, n, groups, F32, bias=False, softplus=False, gate=False, state=False)
+    s.x = Rows(queue, [rng.uniform(0.5, 1, size=(rows, chan))], F32)
+    dy = Rows(queue, [rng.uniform(0.5, 1, size=(rows, chan))], F32)
+    dB, dC = (Rows(queue, [np.zeros((rows, groups * n))], F32, empty=True) for _ in range(2))
+    want, size = (S.selective_scan_grad(**s.of(0), dy=dy.values[0], magnitude=m) for m in (False, True))
+    items = getattr(s, which).values[0].copy()
+    items[at, state] = np.inf
+    setattr(s, which, Rows(queue, [items], F32))
+    dx, ddt = (Rows(queue, [np.zeros((rows, chan))], F32, empty=True) for _ in range(2))
+    fwd = s.plan(keep=True)
+    bwd = seq.plan_selective_scan_grad(queue, fwd, dy.ra, dx.ra, ddt.ra, vec(queue, np.zeros((chan, n))), dB.ra, dC.ra)
+    fwd()
+    bwd()
+    for name, r in (("dB", dB), ("dC", dC)):
+        got = r.get()[0]
+        infinite = np.zeros(got.shape, bool)
+        if name == "dC" and which == "B":
+            infinite[at:, state] = True
+        if name == "dB" and which == "C":
+            infinite[:at + 1, state] = True
+        assert (got[infinite] == np.inf).all()
+        close(got[~infinite], want[name][~infinite], size[name][~infinite], 2 * s.chain(0, chan + rows), F32, name)
+
+
 # ---- norms ---------------------------------------------------------------------------------------
 NORMS = [  # chan, groups, pad, lead, gate, gate_first, residual, weight, scale, norm_weight, Y, H
     (1, 1, 0, 0, True, True, True, True, True, True, True, True),
