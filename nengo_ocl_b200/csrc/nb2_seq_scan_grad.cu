@@ -306,8 +306,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 ? 4 : 3) nb2_selective_sc
           carry[1] = mul2(g1, dec[q + i][1]);
           const f32x2 q0 = mul2(carry[0], q + i ? h[q + i ? q + i - 1 : 0][0] : from[0]);
           const f32x2 q1 = mul2(carry[1], q + i ? h[q + i ? q + i - 1 : 0][1] : from[1]);
-          dA[0] = fma2(q0, s2[0], dA[0]);
-          dA[1] = fma2(q1, s2[0], dA[1]);
+          if (r < rows) {  // (past the end the last state stands before the row: infinite, times a step of zero)
+            dA[0] = fma2(q0, s2[0], dA[0]);
+            dA[1] = fma2(q1, s2[0], dA[1]);
+          }
           float lo, hi;
           unpack2(fma2(g1, b.y, mul2(g0, b.x)), lo, hi);
           pu[i] = lo + hi;

@@ -444,6 +444,26 @@ def test_infinite_weights_of_a_partial_tile(queue, rng, which, chan, groups, n):
         close(got[~infinite], want[name][~infinite], size[name][~infinite], 2 * s.chain(0, chan + rows), F32, name)
 
 
+@pytest.mark.parametrize("rows", [1, 7, 21, 16])
+def test_a_state_that_overflows_in_the_last_row(queue, rng, rows):
+    """The last state stands before no row, so dA does not see it, wherever in a tile the sequence ends."""
+    chan, n = 40, 12
+    s = Scan(queue, rng, [rows], chan, n, 1, F32)
+    dy = Rows(queue, [normal(rng, rows, chan)], F32)
+    want, size = (S.selective_scan_grad(**s.of(0), dy=dy.values[0], magnitude=m) for m in (False, True))
+    B = s.B.values[0].copy()
+    B[-1, 5] = np.inf
+    s.B = Rows(queue, [B], F32)
+    dA = vec(queue, np.full((chan, n), 9.0))
+    outs = [Rows(queue, r.values, F32, empty=True) for r in (s.x, s.dt, s.B, s.C)]
+    fwd = s.plan(keep=True)
+    bwd = seq.plan_selective_scan_grad(queue, fwd, dy.ra, outs[0].ra, outs[1].ra, dA, outs[2].ra, outs[3].ra)
+    fwd()
+    bwd()
+    assert np.isinf(s.new.get()[0][:, 5]).all()
+    close(dA.get(), want["dA"], size["dA"], 2 * s.chain(0, chan + rows), F32, "dA")
+
+
 # ---- norms ---------------------------------------------------------------------------------------
 NORMS = [  # chan, groups, pad, lead, gate, gate_first, residual, weight, scale, norm_weight, Y, H
     (1, 1, 0, 0, True, True, True, True, True, True, True, True),
