@@ -340,6 +340,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 ? 4 : 3) nb2_selective_sc
       }
     }
     __syncwarp();
+    float tile_D = 0.0f, tile_s = 0.0f;  // (a tile's rows apart, then the tiles: shorter chains of additions)
     scan_switch(a.softplus, [&](auto soft) {
       scan_switch(dgate, [&](auto gated) {
 #pragma unroll
@@ -356,12 +357,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 ? 4 : 3) nb2_selective_sc
             put(kDx, tb + r, fmaf(D, dp, sm.ready.sx[r][mine].x * u));
             put(kDdt, tb + r, ds);
             if (decltype(gated)::value) put(kDz, tb + r, gz);
-            dD = fmaf(dp, xv, dD);
-            dbias += ds;
+            tile_D = fmaf(dp, xv, tile_D);
+            tile_s += ds;
           }
         }
       });
     });
+    dD += tile_D;
+    dbias += tile_s;
     if (tb > 0) arrive(stages[cur ^ 1]);
     __syncthreads();
     // the block's share of dB and dC: warps in order

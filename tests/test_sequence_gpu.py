@@ -464,6 +464,25 @@ def test_a_state_that_overflows_in_the_last_row(queue, rng, rows):
     close(dA.get(), want["dA"], size["dA"], 2 * s.chain(0, chan + rows), F32, "dA")
 
 
+def test_sums_over_rows_are_summed_by_tiles(queue, rng, monkeypatch):
+    """dD of a unit of 1008 rows.  Sixteen rows to a tile, 63 tiles, and three more additions: under 90 roundings
+    on the longest chain.  Row after row the same value, 1 + 255 * 2^-23, loses almost half a step with each of the
+    last 496 additions: 250 half steps of the sum."""
+    monkeypatch.setattr(seq, "SCAN_WHOLE_ROWS", 4096)
+    rows, chan, value = 1008, 5, 1 + 255 * 2.0 ** -23
+    s = Scan(queue, rng, [rows], chan, 4, 1, F32, gate=False)
+    s.x = Rows(queue, [np.ones((rows, chan))], F32)
+    dy = Rows(queue, [np.full((rows, chan), value)], F32)
+    outs = [Rows(queue, r.values, F32, empty=True) for r in (s.x, s.dt, s.B, s.C)]
+    dD = vec(queue, np.zeros(chan))
+    fwd = s.plan(keep=True)
+    bwd = seq.plan_selective_scan_grad(queue, fwd, dy.ra, outs[0].ra, outs[1].ra, vec(queue, s.A), outs[2].ra, outs[3].ra, dD=dD)
+    assert bwd.full_args[0].n_units == 1
+    fwd()
+    bwd()
+    close(dD.get(), np.full(chan, rows * value), rows * value, 90, F32, "dD")
+
+
 # ---- norms ---------------------------------------------------------------------------------------
 NORMS = [  # chan, groups, pad, lead, gate, gate_first, residual, weight, scale, norm_weight, Y, H
     (1, 1, 0, 0, True, True, True, True, True, True, True, True),
