@@ -248,6 +248,13 @@ __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_grad_kernel(cons
   for (int64_t tb = t0; tb < t1 + W - 1; tb += kRows, ++group) {
     SeqVecA<T, V> r[2][kRows];
     in.get(tb, group, r);
+    float group_w[W][V], group_b[V];  // (the group's rows apart, then the groups: shorter chains of additions)
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      group_b[v] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < W; ++j) group_w[j][v] = 0.0f;
+    }
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       const int64_t t = tb + i, p = t - (W - 1);
@@ -268,9 +275,9 @@ __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_grad_kernel(cons
       if (t < t1)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          db[v] += gw[W - 1][v];
+          group_b[v] += gw[W - 1][v];
 #pragma unroll
-          for (int j = 0; j < W; ++j) dw[j][v] = fmaf(gw[W - 1][v], xw[j][v], dw[j][v]);
+          for (int j = 0; j < W; ++j) group_w[j][v] = fmaf(gw[W - 1][v], xw[j][v], group_w[j][v]);
         }
       float out[V];
 #pragma unroll
@@ -291,6 +298,12 @@ __global__ void __launch_bounds__(CONV_THREADS) nb2_causal_conv_grad_kernel(cons
       else if (t0 == 0 && p < 0 && dstate)
         o.store(dstate + (p + W - 1) * ds);
     }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      db[v] += group_b[v];
+#pragma unroll
+      for (int j = 0; j < W; ++j) dw[j][v] += group_w[j][v];
+    }
   }
   float* part = a.part + (size_t)unit * (W + 1) * a.channels + c;
 #pragma unroll
@@ -309,11 +322,7 @@ __global__ void __launch_bounds__(256) nb2_conv_grad_sum_kernel(const float* par
   __shared__ float run[8][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t n = (int64_t)(taps + 1) * channels, i = (int64_t)blockIdx.x * 32 + lane;
-  float s = 0.0f;
-  if (i < n)
-#pragma unroll 8
-    for (int u = w; u < n_units; u += 8) s += part[(int64_t)u * n + i];
-  run[w][lane] = s;
+  run[w][lane] = i < n ? nb2_sum_units(part + i, n, n_units, w) : 0.0f;
   __syncthreads();
   if (w == 0 && i < n) {
     float sum = 0.0f;

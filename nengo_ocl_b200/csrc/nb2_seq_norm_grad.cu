@@ -224,11 +224,7 @@ __global__ void __launch_bounds__(256) nb2_norm_grad_sum_kernel(const nb2_residu
   __shared__ float run[8][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t n = 2ll * a.channels, i = (int64_t)blockIdx.x * 32 + lane;
-  float s = 0.0f;
-  if (i < n)
-#pragma unroll 8
-    for (int u = w; u < a.n_units; u += 8) s += a.part[(int64_t)u * n + i];
-  run[w][lane] = s;
+  run[w][lane] = i < n ? nb2_sum_units(a.part + i, n, a.n_units, w) : 0.0f;
   __syncthreads();
   if (w == 0 && i < n) {
     float sum = 0.0f;

@@ -439,11 +439,7 @@ __global__ void __launch_bounds__(256) nb2_scan_grad_sum_kernel(const nb2_select
     part = a.part_d, out = a.dD, at = i - states;
   else if (i < states + 2 * a.channels)
     part = a.part_s, out = a.ddt_bias, at = i - states - a.channels;
-  float s = 0.0f;
-  if (out)
-#pragma unroll 8
-    for (int u = w; u < a.n_units; u += 8) s += part[u * n + at];
-  run[w][lane] = s;
+  run[w][lane] = out ? nb2_sum_units(part + at, n, a.n_units, w) : 0.0f;
   __syncthreads();
   if (w == 0 && out) {
     float sum = 0.0f;

@@ -95,6 +95,26 @@ __device__ __forceinline__ float nb2_silu_slope(float v) {
   return s * (1.0f + v * (1.0f - s));
 }
 
+// A column's share of the sum over units that warp w of 8 adds: every eighth unit in order, 16 of them apart
+// and then these (shorter chains of additions; loads of 16 in flight).  The same result every time.
+__device__ __forceinline__ float nb2_sum_units(const float* column, int64_t pitch, int n_units, int w) {
+  float sum = 0.0f;
+  const float* at = column + w * pitch;
+  int left = (n_units - w + 7) / 8;  // of this warp
+  for (; left >= 16; left -= 16) {
+    float v[16], part = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 16; ++q, at += 8 * pitch) v[q] = *at;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) part += v[q];
+    sum += part;
+  }
+  float part = 0.0f;
+#pragma unroll 8
+  for (int q = 0; q < left; ++q, at += 8 * pitch) part += *at;
+  return sum + part;
+}
+
 // The launch's device must be the calling thread's current one: the pointers belong to it.
 #define NB2_REQUIRE_DEVICE(ordinal)                                                     \
   do {                                                                                  \

@@ -175,6 +175,34 @@ def test_causal_conv_grad(queue, rng, dtype, lengths, chan, taps, pad, lead, sil
     assert np.array_equal(dw.get(), first)
 
 
+def _float32_sum(values):
+    total = np.float32(0)
+    for v in values:
+        total = np.float32(total + v)
+    return total
+
+
+@pytest.mark.parametrize("rows", [64, 1000, 40003])
+def test_order_of_the_sums_over_rows(queue, rng, rows):
+    """dbias (and dw where x is one) without an activation is a plain sum: four rows apart, then a unit's groups
+    of them, every eighth unit in runs of 16, the eight shares.  The float32 additions in that order, to the bit."""
+    chan, taps = 4, 2
+    x, dy = Rows(queue, [np.ones((rows, chan))], F32), Rows(queue, [normal(rng, rows, chan) + 1], F32)
+    y, dx = (Rows(queue, x.values, F32, empty=True) for _ in range(2))
+    dw, db = vec(queue, np.zeros((chan, taps))), vec(queue, np.zeros(chan))
+    fwd = seq.plan_causal_conv(queue, x.ra, vec(queue, np.ones((chan, taps))), y.ra, bias=vec(queue, np.zeros(chan)))
+    bwd = seq.plan_causal_conv_grad(queue, fwd, dy.ra, dx.ra, dw, dbias=db)
+    bwd()
+    unit = bwd.full_args[0].unit_rows
+    assert unit % 4 == 0 and (rows < 40000 or bwd.full_args[0].n_units > 128)
+    for c in range(chan):
+        v = dy.values[0][:, c].astype(np.float32)
+        units = [_float32_sum(_float32_sum(v[i:min(i + 4, t + unit)]) for i in range(t, min(t + unit, rows), 4))
+                 for t in range(0, rows, unit)]
+        shares = [_float32_sum(_float32_sum(units[w::8][i:i + 16]) for i in range(0, len(units[w::8]), 16)) for w in range(8)]
+        assert db.get()[c] == dw.get()[c, 1] == _float32_sum(shares)
+
+
 # ---- selective scan ------------------------------------------------------------------------------
 class Scan:
     """Arguments of a scan at the usual scales, on the device and for the oracle."""
