@@ -175,6 +175,40 @@ def test_causal_conv_grad(queue, rng, dtype, lengths, chan, taps, pad, lead, sil
     assert np.array_equal(dw.get(), first)
 
 
+UNIT_LENGTHS = [[17, 0, 64, 65, 130, 9], [8, 9, 16, 1, 33]]
+
+
+@DTYPES
+@pytest.mark.parametrize("lengths", UNIT_LENGTHS, ids=str)
+@pytest.mark.parametrize("unit_rows", [9, 17, 64])
+@pytest.mark.parametrize("chan,taps,pad,lead,silu", [(136, 4, 8, 16, True), (520, 8, 0, 8, False), (24, 2, 0, 0, True),
+                                                     (33, 3, 1, 1, True)])
+def test_causal_conv_in_long_units(queue, rng, monkeypatch, dtype, lengths, unit_rows, chan, taps, pad, lead, silu):
+    """Units of more rows than a group, as large batches have them: rows copied ahead, several groups to a unit."""
+    monkeypatch.setattr(seq, "_unit_rows", lambda *a: unit_rows)
+    plans = _recorded(monkeypatch, "plan_causal_conv")
+    test_causal_conv(queue, rng, dtype, lengths, chan, taps, pad, lead, silu, True, True)
+    assert plans and all(p.full_args[0].unit_rows == unit_rows for p in plans)
+    assert all(p.full_args[0].vec == (chan != 33) for p in plans[:1])
+
+
+@DTYPES
+@pytest.mark.parametrize("unit_rows", [9, 17, 64])
+@pytest.mark.parametrize("chan,taps,pad,lead,silu", [(136, 4, 8, 16, True), (520, 8, 0, 8, False), (33, 3, 1, 1, True)])
+def test_causal_conv_grad_in_long_units(queue, rng, monkeypatch, dtype, unit_rows, chan, taps, pad, lead, silu):
+    monkeypatch.setattr(seq, "_unit_rows", lambda *a: unit_rows)
+    plans = _recorded(monkeypatch, "plan_causal_conv_grad")
+    test_causal_conv_grad(queue, rng, dtype, UNIT_LENGTHS[0], chan, taps, pad, lead, silu, True, True, True)
+    assert plans and all(p.full_args[0].unit_rows == unit_rows for p in plans)
+
+
+def _recorded(monkeypatch, name):
+    """The plans that ``seq.<name>`` makes from here on."""
+    plans, make = [], getattr(seq, name)
+    monkeypatch.setattr(seq, name, lambda *a, **k: plans.append(make(*a, **k)) or plans[-1])
+    return plans
+
+
 def _float32_sum(values):
     total = np.float32(0)
     for v in values:
@@ -314,6 +348,46 @@ def test_selective_scan_grad(queue, rng, dtype, lengths, chan, n, groups, pad, l
     bwd()
     assert all(np.array_equal(before[0][k], v.get()) for k, v in grads.items())
     assert np.array_equal(before[1], dB.buf.get()) and np.array_equal(before[2], ddt.buf.get())
+
+
+@DTYPES
+@pytest.mark.parametrize("n_seq,chan,n,groups,each", [
+    (131, 1024, 4, 1024, 64),  # (the most sequences of a block, and a last block with the rest)
+    (301, 512, 16, 2, 2), (100, 1000, 128, 1, 6), (40, 1010, 128, 2, 3), (37, 2370, 3, 790, 19)])  # (2368 // 790 tiles: two blocks to a tile)
+@pytest.mark.parametrize("longest", [1, 2])
+def test_tokens_of_many_sequences(queue, rng, dtype, n_seq, chan, n, groups, each, longest):
+    """A block takes several sequences one after the other, the next one's state on its way: 0, 1 or 2 rows each, states
+    in place, in the order of a pool's slots."""
+    lengths = list(rng.randint(0, longest + 1, size=n_seq))
+    lengths[:2] = [longest, 0]
+    s = Scan(queue, rng, lengths, chan, n, groups, dtype)
+    start = s.state.buf.get()
+    plan = s.plan()
+    args = plan.full_args[0]
+    # 16 blocks to each of the 148 multiprocessors; a block takes as many channels as the walk's
+    tiles = groups * -(-(chan // groups) // seq.scan_tile(n))
+    blocks = max(1, min(n_seq, 16 * 148 // tiles))
+    assert args.tokens == 1 and min(-(-n_seq // blocks), 64) == each
+    plan()
+    s.check()
+    y, new = s.y.buf.get(), s.new.buf.get()
+    in_place = s.plan(new_state=s.state.ra)
+    in_place()
+    assert np.array_equal(s.y.buf.get(), y) and np.array_equal(s.state.buf.get(), new)
+    # one sequence by itself: the same additions
+    s.state.buf.set(start)
+    k = int(np.argmax(lengths[5:])) + 5
+    one = lambda r: r.ra[[k]]
+    alone = Rows(queue, [np.zeros((lengths[k], chan))], dtype, empty=True, columns=chan)
+    seq.plan_selective_scan(queue, one(s.x), one(s.dt), s.params["A"], one(s.B), one(s.C), alone.ra, D=s.params["D"],
+                            Z=one(s.z), dt_bias=s.params["dt_bias"], softplus=True, state=one(s.state))()
+    assert np.array_equal(alone.get()[0], s.y.get()[k])
+    # slots of a pool, in another order, in place
+    slots = rng.permutation(n_seq)
+    s.plan(state=s.state.ra[slots], new_state=s.state.ra[slots])()
+    s.state.values = [s.state.values[i] for i in slots]
+    s.new.get = lambda have=s.state.get(): [have[i] for i in slots]
+    s.check()
 
 
 def test_several_sequences_start_from_one_state(queue, rng):
@@ -619,6 +693,30 @@ def test_norm_eps(queue, rng, monkeypatch, dtype, eps, gate_first, chan, groups)
     for f in (seq.plan_residual_norm, S.residual_norm, S.residual_norm_grad):
         monkeypatch.setattr(f, "__defaults__", tuple(eps if d == 1e-5 else d for d in f.__defaults__))
     test_residual_norm(queue, rng, dtype, [3, 0, 2], chan, groups, 0, 0, True, gate_first, True, True, True, True, True, True)
+
+
+@DTYPES
+@pytest.mark.parametrize("chan,groups,pad,lead,gate,gate_first,Y,H", [
+    (64, 8, 0, 0, True, True, True, True), (80, 5, 0, 0, True, False, True, True), (136, 1, 8, 8, True, True, True, True),
+    (1280, 5, 0, 0, True, True, True, True), (1280, 5, 0, 0, False, True, True, False), (1000, 5, 0, 0, True, False, True, True),
+    (1000, 5, 0, 0, True, True, True, False), (1000, 1, 0, 0, True, True, True, False), (33, 3, 1, 1, True, True, False, True),
+    (201, 67, 0, 0, True, False, True, True), (201, 67, 0, 0, True, False, True, False)])
+def test_norm_of_many_rows(queue, rng, monkeypatch, dtype, chan, groups, pad, lead, gate, gate_first, Y, H):
+    """Several rows to a block, as large batches have them: rows on their way in a ring, sums' buffers in turn, gradients
+    summed over the block's rows."""
+    recorded = [_recorded(monkeypatch, "plan_residual_norm"), _recorded(monkeypatch, "plan_residual_norm_grad")]
+    test_residual_norm(queue, rng, dtype, [1301, 0, 300], chan, groups, pad, lead, gate, gate_first, True, True, True, True, Y, H)
+    assert [p[0].full_args[0].unit_rows for p in recorded] == [6, 11]
+
+
+@DTYPES
+@pytest.mark.parametrize("chan,groups,gate_first", [(3000, 5, True), (6000, 1, False), (9001, 1, True), (12000, 125, False),
+                                                    (20000, 4, True), (32768, 1, True)])
+def test_wide_norm_of_many_rows(queue, rng, monkeypatch, dtype, chan, groups, gate_first):
+    """The same with several vectors to a thread; above 16384 channels (16 bits: 8192) the gradients are summed in memory."""
+    recorded = [_recorded(monkeypatch, "plan_residual_norm"), _recorded(monkeypatch, "plan_residual_norm_grad")]
+    test_residual_norm(queue, rng, dtype, [150, 0, 147], chan, groups, 0, 0, True, gate_first, True, True, True, True, True, True)
+    assert [p[0].full_args[0].unit_rows for p in recorded] == [2, 3]
 
 
 def test_norm_infinite_weight_stays_in_its_channel(queue, rng):
