@@ -28,6 +28,8 @@ __device__ __forceinline__ ScanPlace scan_place(const int64_t* table, int n_seq,
   return {table[(size_t)(1 + 2 * array) * n_seq + k], table[(size_t)(2 + 2 * array) * n_seq + k]};
 }
 
+// The hardware's exponential: 2 units in the last place, results below 2^-126 are zero (a state that decays by that in
+// a row has forgotten).  The rounded row-by-row products it goes into carry more: an exact one moves no output's error.
 __device__ __forceinline__ float scan_exp2(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -36,7 +38,9 @@ __device__ __forceinline__ float scan_exp2(float v) {
 
 // log(1 + e^v) = max(v, 0) + log1p(e), e = exp(-|v|) in [0, 1], without a branch, so that a lane's rows overlap.
 // log1p(e) = 2 atanh(w), w = e / (2 + e) <= 1/3: the series in w^2 <= 1/9 to w^12 leaves 2e-8 of it, and small e
-// (a step size of 0.001 is log1p(0.001)) keep their digits.
+// (a step size of 0.001 is log1p(0.001)) keep their digits.  The argument's rounding in base 2 makes e uncertain by
+// |v| * 2^-24; expf in its place leaves every output's error as it is and costs 6 us of 225 (4097 rows of prompts x 4096
+// channels x 16 states) and 8 of 423 (training, 4096 x 2048 x 16).
 __device__ __forceinline__ float scan_softplus(float v) {
   const float e = scan_exp2(-LOG2E * fabsf(v));
   const float w = __fdividef(e, 2.0f + e), q = w * w;

@@ -7,7 +7,10 @@ step) and ``plan_conv2d``; the reference has no counterpart.  A *sequence array*
 lengths may differ and may be zero.  Rows may be any distance apart (an item can be a column range of a
 wider buffer), channels lie next to each other.  Element types: float32, float16 and ``bfloat16`` (one
 for all sequence arrays of a plan).  Parameters, scan states and their gradients are float32; sums,
-states and norms are held in float32 whatever the type, and results are rounded once, when stored.
+states and norms are held in float32 whatever the type, and results are rounded once, when stored.  The
+exponentials of gates, steps and decays are the hardware's, for float32 too: a gate's sigmoid is off by up to
+(4 + 1.2 |v|) * 2^-23 of its value.  An infinite or NaN input may make NaN of whatever depends on it, and of nothing
+else: other sequences, earlier rows (backward: later ones) and the scan's other channels are as without it.
 
 The same plan serves prompts and single tokens: state goes in through ``state`` and comes out through
 ``new_state``, which may be the same items (updated in place).  Otherwise nothing that a plan writes may
