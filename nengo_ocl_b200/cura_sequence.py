@@ -129,6 +129,7 @@ class _Arguments:
         self.fields = []
         self.kept = []
         self.blocks = []
+        self.scratched = 0
         self.aligned = True
 
     def rows(self, name, ra, columns=None, lengths=None, dtype=None, written=False, optional=False, vec=True):
@@ -259,8 +260,14 @@ class _Arguments:
         host = np.ascontiguousarray(np.stack([seq, first], axis=1).astype(np.int32))
         return self._need(host.nbytes, host), len(seq)
 
-    def scratch(self, n):
+    def scratch(self, n, passes=2):
+        """``n`` floats, read or written ``passes`` times in all."""
+        self.scratched += 4 * int(n) * passes
         return self._need(4 * max(int(n), 1))
+
+    def moved(self):
+        """Bytes that a call moves: every array's once, and the scratch's."""
+        return sum(int((m.rows * m.width).sum()) for m in self.memory) + self.scratched
 
     def place(self, args, **tokens):
         """Allocates what was asked for and sets the fields ``name=token`` of ``args``."""
@@ -299,10 +306,6 @@ def _make_plan(queue, name, entry, args, kept, gsize, n_launches, tag, flops, mo
     plan.flops_per_call = int(flops)
     plan.bw_per_call = int(moved)
     return plan
-
-
-def _nbytes(memory):
-    return sum(int((m.rows * m.width).sum()) for m in memory)
 
 
 def _unit_rows(total, tiles, least, want):
@@ -344,7 +347,7 @@ def plan_causal_conv(queue, X, W, Y, bias=None, state=None, new_state=None, acti
     units, args.n_units = a.units(args.unit_rows)
     a.place(args, table=a.table(), units=units)
     plan = _make_plan(queue, "cura_causal_conv", "nb2_causal_conv", args, a.kept, args.n_units * a.channels, 1, tag,
-                      total * a.channels * (2 * taps + 4), _nbytes(a.memory))
+                      total * a.channels * (2 * taps + 4), a.moved())
     plan.sequence_args = dict(X=X, W=W, bias=bias, state=state, new_state=new_state, activation=activation)
     return plan
 
@@ -378,7 +381,6 @@ def plan_causal_conv_grad(queue, plan, dY, dX, dW, dbias=None, dstate=None, dnew
         dbias=a.param("dbias", dbias, (a.channels,), written=True, optional=True),
         taps=taps, silu=int(f["activation"] == "silu"), **a.common())
     a.check_overlaps()
-    moved = _nbytes(a.memory)
     width = 16 // a.dtype.itemsize
     args.vec = int(a.aligned and a.channels % width == 0)
     total = int(a.lengths.sum())
@@ -386,7 +388,7 @@ def plan_causal_conv_grad(queue, plan, dY, dX, dW, dbias=None, dstate=None, dnew
     units, args.n_units = a.units(args.unit_rows)
     a.place(args, table=a.table(), units=units, part=a.scratch(args.n_units * (taps + 1) * a.channels))
     return _make_plan(queue, "cura_causal_conv_grad", "nb2_causal_conv_grad", args, a.kept,
-                      args.n_units * a.channels, 2, tag, total * a.channels * (6 * taps + 10), moved)
+                      args.n_units * a.channels, 2, tag, total * a.channels * (6 * taps + 10), a.moved())
 
 
 # ---- selective state space scan --------------------------------------------------------------
@@ -415,7 +417,7 @@ def _scan_units(a, args, tiles, row, work, twice):
     tokens = dict.fromkeys(("units", "ends", "sums"))
     tokens["units"], args.n_units = a.units(args.unit_rows)
     if args.n_units > len(a.lengths):
-        tokens["ends"] = a.scratch(args.n_units * a.channels * args.n_states)
+        tokens["ends"] = a.scratch(args.n_units * a.channels * args.n_states, passes=4)  # (the join reads and writes it)
         tokens["sums"] = a.scratch(args.n_units * a.channels)
     return np.cumsum(units) - units, tokens
 
@@ -465,10 +467,9 @@ def plan_selective_scan(queue, X, dt, A, B, C, Y, D=None, Z=None, dt_bias=None, 
     args.D = a.param("D", D, (a.channels,), optional=True)
     args.dt_bias = a.param("dt_bias", dt_bias, (a.channels,), optional=True)
     a.check_overlaps(in_place=("state", "new_state"))
-    moved = _nbytes(a.memory)
     blocks = -(-a.lengths // KEEP_ROWS)
     first = np.cumsum(blocks) - blocks
-    kept = a.scratch(int(blocks.sum()) * a.channels * n) if keep else None
+    kept = a.scratch(int(blocks.sum()) * a.channels * n, passes=1) if keep else None
     longest = int(a.lengths.max())
     args.tokens = int(longest <= TOKEN_ROWS and not keep)
     launches, first_unit, tokens = 1, np.arange(len(a.lengths)), {}
@@ -479,7 +480,7 @@ def plan_selective_scan(queue, X, dt, A, B, C, Y, D=None, Z=None, dt_bias=None, 
     a.place(args, table=a.table(first, first_unit), keep=kept, **tokens)
     total = int(a.lengths.sum())
     plan = _make_plan(queue, "cura_selective_scan", "nb2_selective_scan", args, a.kept, len(a.lengths) * a.channels,
-                      launches, tag, total * a.channels * (7 * n + 20), moved)
+                      launches, tag, total * a.channels * (7 * n + 20), a.moved())
     plan.sequence_args = dict(X=X, dt=dt, A=A, B=B, C=C, D=D, Z=Z, dt_bias=dt_bias, softplus=bool(softplus), state=state,
                               keep=args.keep, kept=a.kept, first=first, n=n, groups=groups)
     return plan
@@ -525,8 +526,8 @@ def plan_selective_scan_grad(queue, plan, dY, dX, ddt, dA, dB, dC, dD=None, dZ=N
     args.dD = a.param("dD", dD, (a.channels,), written=True, optional=True)
     args.ddt_bias = a.param("ddt_bias", ddt_bias, (a.channels,), written=True, optional=True)
     a.check_overlaps()
-    moved = _nbytes(a.memory)
     args.keep = f["keep"]
+    a.scratched += 4 * int((-(-a.lengths // KEEP_ROWS)).sum()) * a.channels * n
     a.kept.append(f["kept"])
     total = int(a.lengths.sum())
     args.total_rows = total
@@ -536,7 +537,7 @@ def plan_selective_scan_grad(queue, plan, dY, dX, ddt, dA, dB, dC, dD=None, dZ=N
             part_bc=a.scratch(tiles * total * 2 * width), part_a=a.scratch(args.n_units * a.channels * n),
             part_d=a.scratch(args.n_units * a.channels), part_s=a.scratch(args.n_units * a.channels), **tokens)
     return _make_plan(queue, "cura_selective_scan_grad", "nb2_selective_scan_grad", args, a.kept,
-                      len(a.lengths) * a.channels, 3 + 2 * bool(args.ends), tag, total * a.channels * (19 * n + 30), moved)
+                      len(a.lengths) * a.channels, 3 + 2 * bool(args.ends), tag, total * a.channels * (19 * n + 30), a.moved())
 
 
 # ---- norms around a block --------------------------------------------------------------------
@@ -577,7 +578,6 @@ def plan_residual_norm(queue, X, Y=None, H=None, gate=None, gate_first=True, res
         norm_weight=a.param("norm_weight", norm_weight, (a.channels,), optional=True),
         groups=groups, gate_first=int(bool(gate_first)), eps=float(eps), **a.common())
     a.check_overlaps()
-    moved = _nbytes(a.memory)
     args.vec = int(a.aligned and (a.channels // groups) % (16 // a.dtype.itemsize) == 0)
     args.param_vec = int(not any(p % 16 for p in (args.weight, args.scale, args.norm_weight) if p))
     total = int(a.lengths.sum())
@@ -585,7 +585,7 @@ def plan_residual_norm(queue, X, Y=None, H=None, gate=None, gate_first=True, res
     units, args.n_units = a.units(args.unit_rows)
     a.place(args, table=a.table(), units=units)
     plan = _make_plan(queue, "cura_residual_norm", "nb2_residual_norm", args, a.kept, total * a.channels, 1, tag,
-                      total * a.channels * 16, moved)
+                      total * a.channels * 16, a.moved())
     plan.sequence_args = dict(X=X, gate=gate, gate_first=gate_first, residual=residual, weight=weight, scale=scale,
                               norm_weight=norm_weight, groups=groups, eps=eps)
     return plan
@@ -623,7 +623,6 @@ def plan_residual_norm_grad(queue, plan, dX, dY=None, dH=None, dgate=None, dresi
         dnorm_weight=a.param("dnorm_weight", dnorm_weight, vector, written=True, optional=True),
         groups=f["groups"], gate_first=int(bool(f["gate_first"])), eps=float(f["eps"]), **a.common())
     a.check_overlaps()
-    moved = _nbytes(a.memory)
     args.vec = int(a.aligned and (a.channels // f["groups"]) % (16 // a.dtype.itemsize) == 0)
     args.param_vec = int(not any(p % 16 for p in (args.weight, args.scale, args.norm_weight) if p))
     total = int(a.lengths.sum())
@@ -631,4 +630,4 @@ def plan_residual_norm_grad(queue, plan, dX, dY=None, dH=None, dgate=None, dresi
     units, args.n_units = a.units(args.unit_rows)
     a.place(args, table=a.table(), units=units, part=a.scratch(args.n_units * 2 * a.channels))
     return _make_plan(queue, "cura_residual_norm_grad", "nb2_residual_norm_grad", args, a.kept, total * a.channels,
-                      2, tag, total * a.channels * 40, moved)
+                      2, tag, total * a.channels * 40, a.moved())

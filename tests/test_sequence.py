@@ -363,6 +363,22 @@ def test_column_ranges_of_one_buffer_are_accepted(fake_queue):
         case.forward("norm", Y=left, H=_again(both, shape1s=[8] * 3, starts=both.starts + 7))
 
 
+def test_bytes_of_a_call_count_its_scratch(fake_queue):
+    """40 rows of 8 channels x 4 states: 8 float32 vectors, 3 states kept, one channel tile's share of dB and dC."""
+    case = Case(fake_queue, lengths=(40,))
+    rows, state, params = 4 * 40 * 8, 4 * 8 * 4, 4 * (8 * 4 + 8 + 8)
+    fwd = case.forward("scan")
+    assert fwd.bw_per_call == 6 * rows + 2 * state + params + 3 * state   # (X, dt, B, C, Y, Z)
+    bwd = case.backward("scan", fwd)
+    units = 2 * (state + 2 * 4 * 8) * bwd.full_args[0].n_units           # shares of dA, dD and ddt_bias
+    assert bwd.full_args[0].n_units == 1
+    assert bwd.bw_per_call == 11 * rows + 2 * state + 2 * params + 3 * state + 2 * (4 * 40 * 2 * 8) + units
+    fwd = case.forward("conv")
+    assert fwd.bw_per_call == 2 * rows + 2 * 4 * 3 * 8 + 4 * 8 * 5
+    bwd = case.backward("conv", fwd)
+    assert bwd.bw_per_call == 3 * rows + 3 * 4 * 3 * 8 + 2 * 4 * 8 * 5 + 2 * 4 * 8 * 5 * bwd.full_args[0].n_units
+
+
 def test_gradients_without_their_argument_are_refused(fake_queue):
     case = Case(fake_queue)
     for kind, name, grad in (("conv", "bias", "dbias"), ("conv", "state", "dstate"), ("scan", "D", "dD"),
