@@ -153,23 +153,22 @@ class _Arguments:
         if (ra.shape1s != columns).any():
             raise ValueError("%s: %d columns are expected" % (name, columns))
         starts, strides = ra.index64("starts"), ra.index64("stride0s")
-        rows = np.broadcast_to(lengths, starts.shape)
+        rows, some = lengths, lengths > 0
         strides = np.where(rows > 1, strides, columns)
-        if columns > 1 and ((ra.index64("stride1s") != 1) & (rows > 0)).any():
+        if columns > 1 and ((ra.index64("stride1s") != 1) & some).any():
             raise NotImplementedError("%s: channels must lie next to each other (stride1 == 1)" % name)
         if (strides < 0).any():
             raise NotImplementedError("%s: rows in reverse order" % name)
         ends = starts + np.maximum(rows - 1, 0) * strides + columns
-        if ((rows > 0) & ((starts < 0) | (ends > ra.cl_buf.size))).any():
+        if (some & ((starts < 0) | (ends > ra.cl_buf.size))).any():
             raise ValueError("%s: an item reaches past the end of its buffer" % name)
         self._same_device(name, ra.cl_buf)
         size = dtype.itemsize
         self.memory.append(_Memory(name, ra.cl_buf.data + starts * size, rows, strides * size,
                                    np.full(len(starts), columns * size), written))
         if vec:
-            used = rows > 0
-            self.aligned &= not (ra.cl_buf.data % 16 or (starts[used] * size % 16).any()
-                                 or (strides[used & (rows > 1)] * size % 16).any())
+            self.aligned = self.aligned and not (ra.cl_buf.data % 16 or (starts[some] * size % 16).any()
+                                                 or (strides[rows > 1] * size % 16).any())
         self.fields += [starts, strides]
         self.kept.append(ra.cl_buf)
         return ra.cl_buf.data

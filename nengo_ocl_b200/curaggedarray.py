@@ -60,12 +60,14 @@ class _LazyIndex:
         return arr
 
     def __set__(self, obj, values):
-        wide = np.array(values, dtype=np.int64)
-        wide.setflags(write=False)
-        arr = wide.astype(np.int32)
+        wide = None
+        if getattr(values, "dtype", None) != np.int32:
+            values = wide = np.array(values, dtype=np.int64)
+            wide.setflags(write=False)
+        arr = np.array(values, dtype=np.int32)
         arr.setflags(write=False)
-        obj.__dict__["_wide_" + self.name] = wide
-        obj.__dict__["_" + self.name] = arr if np.array_equal(arr, wide) else None
+        obj.__dict__["_wide_" + self.name] = wide  # (None: as in 32 bits)
+        obj.__dict__["_" + self.name] = arr if wide is None or (arr == wide).all() else None
         obj.__dict__.pop("_cl_" + self.name, None)
         obj.__dict__["_sizes"] = None
 
@@ -108,7 +110,8 @@ class CUDARaggedArray:
 
     def index64(self, name):
         """``starts``, ``stride0s`` ... in 64 bits, whatever their values."""
-        return self.__dict__["_wide_" + name]
+        wide = self.__dict__["_wide_" + name]
+        return self.__dict__["_" + name].astype(np.int64) if wide is None else wide
 
     def _device_index(self, name):
         key = "_cl_" + name
