@@ -142,8 +142,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, VEC ? 6 : 4) nb2_selective_scan_
         const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&st.bc[r0 + i][0][l.n0]);
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-          d[i][p][0] = exp2x2(mul2(s2[p], A2[p][0]));
-          d[i][p][1] = exp2x2(mul2(s2[p], A2[p][1]));
+          d[i][p][0] = scan_decay2(s2[p], A2[p][0]);
+          d[i][p][1] = scan_decay2(s2[p], A2[p][1]);
           u[i][p][0] = mul2(x2[p], b.x);
           u[i][p][1] = mul2(x2[p], b.y);
         }
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 8) nb2_selective_scan_token_kern
         const float sx = step * s.x[u];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          s.h[u][m] = fmaf(scan_exp2(step * A2[u][m]), s.h[u][m], sx * s.b[m]);
+          s.h[u][m] = fmaf(scan_decay(step, A2[u][m]), s.h[u][m], sx * s.b[m]);
           o = fmaf(s.c[m], s.h[u][m], o);
         }
 #pragma unroll

@@ -20,6 +20,7 @@ struct ScanGradSmem {
   ScanArray arrays[kArrays];
   ScanRows<S, 1, R> ready;
   float dp[R][ScanRows<S, 1, R>::kPitch];
+  float4 kept[2][SCAN_THREADS];  // the lanes' states before a tile, of this one and the next
   float4 sums[R][SCAN_THREADS / S];  // over the states: g B, g a h[t-1] A log2(e), C h
   alignas(16) float red[R][SCAN_WARPS][8 * S];  // dB, dC of a row: a warp's channels added
 };
@@ -131,8 +132,8 @@ __global__ void __launch_bounds__(SCAN_THREADS) nb2_scan_grad_ends_kernel(const 
       const float2 sd = ready.sx[r][mine];
       const f32x2 s2 = pack2(sd.x, sd.x), d2 = pack2(sd.y, sd.y);
       const ulonglong2 cw = *reinterpret_cast<const ulonglong2*>(&st.bc[r][1][l.n0]);
-      g[0] = mul2(exp2x2(mul2(s2, A2[0])), fma2(cw.x, d2, g[0]));
-      g[1] = mul2(exp2x2(mul2(s2, A2[1])), fma2(cw.y, d2, g[1]));
+      g[0] = mul2(scan_decay2(s2, A2[0]), fma2(cw.x, d2, g[0]));
+      g[1] = mul2(scan_decay2(s2, A2[1]), fma2(cw.y, d2, g[1]));
     }
     if (tb > 0) arrive(stages[cur ^ 1]);
   }
@@ -196,7 +197,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 ? 4 : 3) nb2_selective_sc
   const bool stores = l.valid(0) && l.j < RB;
   // A lane without a channel adds nothing to dB and dC: steps, gradients, weights and states of zero.
   const int bc0 = l.valid(0) ? l.n0 : 4 * S;
-  float dD = 0.0f, dbias = 0.0f, h0[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  float dD = 0.0f, dbias = 0.0f;
+  sm.kept[0][tid] = sm.kept[1][tid] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // (only real states are written)
   scan_clear_weights(stages, 2);
   __syncthreads();
   ScanWeights<VEC, T, S, R> weights(n);
@@ -210,7 +212,17 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 ? 4 : 3) nb2_selective_sc
       }
     const ScanArray b = sm.arrays[kB], c = sm.arrays[kC];
     weights.load((const T*)b.p + from * b.stride, b.stride, (const T*)c.p + from * c.stride, c.stride, n, rows);
-    if (l.valid(0)) scan_load4(keep + from / R * a.channels * n, l.n0, n, n % 4 == 0, h0);
+    if (l.valid(0)) {
+      const float* k = keep + from / R * a.channels * n + l.n0;
+      float* to = reinterpret_cast<float*>(&sm.kept[&st - stages][tid]);
+      if (n % 4 == 0) {
+        if (l.n0 < n) scan_cp_async(to, k, 16);
+      } else {
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          if (l.n0 + m < n) scan_cp_async4(to + m, k + m);
+      }
+    }
   };
   auto arrive = [&](Stage& st) {
     weights.store(st.bc);
@@ -232,7 +244,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 ? 4 : 3) nb2_selective_sc
     scan_cp_wait();
     __syncthreads();
     const Stage& st = stages[cur];
-    const f32x2 start[2] = {pack2(h0[0], h0[1]), pack2(h0[2], h0[3])};
+    const ulonglong2& start = *reinterpret_cast<const ulonglong2*>(&sm.kept[cur][tid]);
     if (tb > 0) fetch(stages[cur ^ 1], tb - R, R);
     scan_switch(a.softplus, [&](auto soft) {
       scan_switch(gate, [&](auto gated) {
@@ -264,27 +276,27 @@ __global__ void __launch_bounds__(SCAN_THREADS, S < 16 ? 4 : 3) nb2_selective_sc
     // (The later half's start costs its rows' decays once more, which the registers for 16 rows would cost in
     // resident warps.)
     constexpr int H = R / 2;
-    f32x2 mid[2] = {start[0], start[1]};
+    f32x2 mid[2] = {start.x, start.y};
     if (rows > H)
 #pragma unroll
       for (int r = 0; r < H; ++r) {
         f32x2 s2[1], x2[1];
         sm.ready.get(r, mine, s2, x2);
         const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&st.bc[r][0][bc0]);
-        mid[0] = fma2(exp2x2(mul2(s2[0], A2[0])), mid[0], mul2(x2[0], b.x));
-        mid[1] = fma2(exp2x2(mul2(s2[0], A2[1])), mid[1], mul2(x2[0], b.y));
+        mid[0] = fma2(scan_decay2(s2[0], A2[0]), mid[0], mul2(x2[0], b.x));
+        mid[1] = fma2(scan_decay2(s2[0], A2[1]), mid[1], mul2(x2[0], b.y));
       }
 #pragma unroll 1
     for (int rb = rows > H ? H : 0; rb >= 0; rb -= H) {
-      const f32x2 from[2] = {rb ? mid[0] : start[0], rb ? mid[1] : start[1]};
+      const f32x2 from[2] = {rb ? mid[0] : start.x, rb ? mid[1] : start.y};
       f32x2 h[H][2], dec[H][2];
 #pragma unroll
       for (int i = 0; i < H; ++i) {
         f32x2 s2[1], x2[1];
         sm.ready.get(rb + i, mine, s2, x2);
         const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&st.bc[rb + i][0][bc0]);
-        dec[i][0] = exp2x2(mul2(s2[0], A2[0]));
-        dec[i][1] = exp2x2(mul2(s2[0], A2[1]));
+        dec[i][0] = scan_decay2(s2[0], A2[0]);
+        dec[i][1] = scan_decay2(s2[0], A2[1]);
         h[i][0] = fma2(dec[i][0], i ? h[i ? i - 1 : 0][0] : from[0], mul2(x2[0], b.x));
         h[i][1] = fma2(dec[i][1], i ? h[i ? i - 1 : 0][1] : from[1], mul2(x2[0], b.y));
       }

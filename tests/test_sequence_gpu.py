@@ -585,6 +585,31 @@ def test_sums_over_rows_are_summed_by_tiles(queue, rng, monkeypatch):
     close(dD.get(), np.full(chan, rows * value), rows * value, 90, F32, "dD")
 
 
+def test_decays_are_right_on_average(queue, rng, monkeypatch):
+    """A state that only decays, over 2048 rows of exponents between -0.04 and -0.02: the decays' mean error counts
+    2048 times.  A mean of at most 0.2 half steps, and 0.7 of them at random (the exponential 0.53, the product's
+    rounding 0.29, the exponent's less) six times sqrt(2048): 600.  Off by 0.45 on average it would be 900."""
+    monkeypatch.setattr(seq, "SCAN_WHOLE_ROWS", 4096)
+    rows, chan, n = 2048, 16, 4
+    s = Scan(queue, rng, [rows], chan, n, 1, F32, bias=False, softplus=False, gate=False)
+    s.A = -np.ones((chan, n), np.float32)
+    s.params["A"] = vec(queue, s.A)
+    s.dt = Rows(queue, [np.log(2) * rng.uniform(0.02, 0.04, size=(rows, chan))], F32)
+    s.x = Rows(queue, [np.zeros((rows, chan))], F32)
+    dy, dnew = Rows(queue, [np.zeros((rows, chan))], F32), Rows(queue, [normal(rng, chan, n)], F32)
+    outs = [Rows(queue, r.values, F32, empty=True) for r in (s.x, s.dt, s.B, s.C)]
+    dstate = Rows(queue, [np.zeros((chan, n))], F32, empty=True)
+    fwd = s.plan(keep=True)
+    bwd = seq.plan_selective_scan_grad(queue, fwd, dy.ra, outs[0].ra, outs[1].ra, vec(queue, s.A), outs[2].ra, outs[3].ra,
+                                       dstate=dstate.ra, dnew_state=dnew.ra)
+    assert fwd.full_args[0].n_units == bwd.full_args[0].n_units == 1
+    fwd()
+    bwd()
+    decay = np.exp(-s.dt.values[0].sum(0))[:, None]
+    for got, start in ((s.new, s.state), (dstate, dnew)):
+        close(got.get()[0], decay * start.values[0], np.abs(decay * start.values[0]), 600, F32, "decayed")
+
+
 # ---- norms ---------------------------------------------------------------------------------------
 NORMS = [  # chan, groups, pad, lead, gate, gate_first, residual, weight, scale, norm_weight, Y, H
     (1, 1, 0, 0, True, True, True, True, True, True, True, True),
