@@ -110,8 +110,12 @@ class CUDARaggedArray:
 
     def index64(self, name):
         """``starts``, ``stride0s`` ... in 64 bits, whatever their values."""
+        return self._places(name).astype(np.int64, copy=False)
+
+    def _places(self, name):
+        """The same as it is kept: in 32 bits where the values came so (no copy)."""
         wide = self.__dict__["_wide_" + name]
-        return self.__dict__["_" + name].astype(np.int64) if wide is None else wide
+        return self.__dict__["_" + name] if wide is None else wide
 
     def _device_index(self, name):
         key = "_cl_" + name
@@ -166,7 +170,7 @@ class CUDARaggedArray:
         self.cl_buf = to_device(self.queue, buf)
 
     def __len__(self):
-        return len(self.index64("starts"))
+        return len(self._places("starts"))
 
     def __str__(self):
         out = StringIO()
@@ -180,9 +184,9 @@ class CUDARaggedArray:
         if is_iterable(item) or isinstance(item, slice):
             return self.getitem_device(item)
         item = int(item)
-        buf = to_host(self.queue, self.cl_buf, self.dtype, self.index64("starts")[item],
+        buf = to_host(self.queue, self.cl_buf, self.dtype, self._places("starts")[item],
                       (self.shape0s[item], self.shape1s[item]),
-                      (self.index64("stride0s")[item], self.index64("stride1s")[item]))
+                      (self._places("stride0s")[item], self._places("stride1s")[item]))
         buf.setflags(write=False)
         return buf
 
@@ -192,14 +196,14 @@ class CUDARaggedArray:
         if is_iterable(item):
             item = np.asarray([int(i) for i in item], dtype=np.intp)
             return CUDARaggedArray.from_buffer(
-                self.queue, self.cl_buf, self.index64("starts")[item], self.shape0s[item], self.shape1s[item],
-                self.index64("stride0s")[item], self.index64("stride1s")[item], names=[self.names[i] for i in item])
+                self.queue, self.cl_buf, self._places("starts")[item], self.shape0s[item], self.shape1s[item],
+                self._places("stride0s")[item], self._places("stride1s")[item], names=[self.names[i] for i in item])
         item = int(item)
         isz = self.dtype.itemsize
         arr = DeviceArray(self.queue, (self.shape0s[item], self.shape1s[item]), self.dtype,
                           data=self.cl_buf.base_data,
-                          offset=self.cl_buf.offset + int(self.index64("starts")[item]) * isz, base=self.cl_buf)
-        arr.strides = (int(self.index64("stride0s")[item]) * isz, int(self.index64("stride1s")[item]) * isz)
+                          offset=self.cl_buf.offset + int(self._places("starts")[item]) * isz, base=self.cl_buf)
+        arr.strides = (int(self._places("stride0s")[item]) * isz, int(self._places("stride1s")[item]) * isz)
         return arr
 
     def __setitem__(self, item, new_value):
@@ -207,8 +211,8 @@ class CUDARaggedArray:
             raise NotImplementedError("assigning to several items at once is not supported")
         item = int(item)
         m, n = int(self.shape0s[item]), int(self.shape1s[item])
-        sm, sn = int(self.index64("stride0s")[item]), int(self.index64("stride1s")[item])
-        start = int(self.index64("starts")[item])
+        sm, sn = int(self._places("stride0s")[item]), int(self._places("stride1s")[item])
+        start = int(self._places("starts")[item])
         if m * n == 0:
             return
         if self.dtype == bfloat16 or is_bfloat16(new_value):
@@ -237,8 +241,8 @@ class CUDARaggedArray:
 
     def to_host(self):
         """Copy the whole object to a host RaggedArray."""
-        return RaggedArray.from_buffer(self.buf, self.index64("starts"), self.shape0s, self.shape1s,
-                                       self.index64("stride0s"), self.index64("stride1s"), names=self.names)
+        return RaggedArray.from_buffer(self.buf, self._places("starts"), self.shape0s, self.shape1s,
+                                       self._places("stride0s"), self._places("stride1s"), names=self.names)
 
 
 # The reference's name, so planning code written against it imports unchanged.
