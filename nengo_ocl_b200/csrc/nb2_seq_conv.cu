@@ -5,7 +5,7 @@
 // Rows before the first one come from the state, which is also a sequence's last W - 1 rows.
 //
 // Memory would allow 20 us for 8192 rows x 4096 channels in bfloat16; the kernel takes 40: with 4 taps and the silu a value
-// is 16 instructions, and the window and weights of four channels leave 20 warps to a multiprocessor.  Eight
+// is 30 instructions (counted; 0.72 of the issue slots), and the window and weights of four channels leave 24 warps to a multiprocessor (float32: 20).  Eight
 // channels to a thread 47 us, weights read from memory by each thread 54, one row at a time 81.
 #include "nb2_sequence.cuh"
 

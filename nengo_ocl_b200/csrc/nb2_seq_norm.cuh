@@ -4,7 +4,7 @@
 // (the gate before or after the first norm, every part optional), and the backward pass.  Bound by memory: a
 // block holds a whole row in registers, NV vectors of V channels to a thread, so each array is read or
 // written once, and all of a row's loads are in flight before its first sum is needed.  Measured (B200, bfloat16): 8192 rows
-// x 4096, all parts, 70 us = 4.8 TB/s, 0.73 of the copy rate (without the copies ahead 110); backward 88 us for 4096
+// x 4096, all parts, 70 us = 4.8 TB/s, 0.73 of the copy rate (without the copies ahead 110); backward 87 us for 4096
 // rows, 3.0 TB/s: its sums hold a block of 512 threads a multiprocessor, whose four phases a row do not overlap.
 #pragma once
 #include "nb2_sequence.cuh"

@@ -9,11 +9,12 @@
 // A tile of R rows is worked in three phases, each a warp's own: its lanes prepare (s, s x) of the tile's rows
 // for their channels, walk the rows through the states, and finish the outputs.
 //
-// Bound by the special function unit: n + 4 results a row and channel at 16 a cycle and multiprocessor, 25 us for
+// Bound by the special function unit: n + 4 results a row and channel at 16 a cycle and multiprocessor, 19 us for
 // 4096 rows x 1024 channels x 16 states and walk where memory needs 10 (float32).  Measured (B200): 48 x 256 rows x 4096
-// channels 326 us, 0.7 of the unit busy (231 us of it at full rate); 4097 rows of 4 uneven prompts, split, 226 us. Six
-// blocks a multiprocessor (80 registers) against five and four: 226 / 231 / 231 us; rows copied element by
-// element need more registers: four.
+// channels 326 us, 0.7 of the unit busy (225 us of it at full rate); 4097 rows of 4 uneven prompts, split, 225 us.  Bounds
+// of six blocks a multiprocessor (80 registers; float32's shared memory, 41 KB, holds five, 16 bits' 28 KB six) against
+// five and four: 225 / 230 / 231 us, one bfloat16 prompt of 16384 x 1024 210 / 210 / 213; rows copied element by element
+// need more registers: four.
 #define SCAN_P 2
 #define SCAN_TOKEN_BLOCKS 16
 template <typename T, int S, bool VEC, bool ENDS>

@@ -11,8 +11,9 @@
 //
 // Bound by shared-memory words and issue slots: a lane reads 26 words a row (B and C twice, the prepared rows) and the
 // sums over channels and states are 9 shuffles.  Measured (B200, 2 x 2048 rows x 2048 channels x 16 states, float32): both
-// passes 427 us, of which this walk about 230; 16 x 512 rows 654.  Four blocks a multiprocessor against three and five:
-// 427 / 456 / 477 us; above 32 states three: 543 against 617 with four.  Two channels to a lane spill: 466.
+// passes 424 us, of which this walk about 225; 16 x 512 rows 652.  Four blocks a multiprocessor against three and five:
+// 424 / 456 / 483 us; above 32 states three (64 states 2.22 ms against 2.27 with four).  Two channels to a lane spilled,
+// which an earlier form of this walk paid with a tenth.
 enum ScanGradArrays { kDt, kX, kDy, kZ, kB, kC, kDx, kDdt, kDz, kArrays };
 template <int S>
 struct ScanGradSmem {

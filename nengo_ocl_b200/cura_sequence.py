@@ -40,17 +40,18 @@ MEM_UNKNOWN, MEM_DEVICE = 0, 2  # NB2_MEM_*
 
 # Launch shapes, chosen by measurement on a B200 (148 multiprocessors).
 # Units a multiprocessor of the convolution (rows of a unit are halved, 64 to 8, until there are so many): 2 / 4 / 8 / 16
-# units 44.6 / 44.9 / 41.5 / 45.0 us forward (8192 rows x 4096, bf16), 2 / 4 / 8 54.8 / 57.5 / 57.3 us for both passes
+# units 42.9 / 43.1 / 40.1 / 43.4 us forward (8192 rows x 4096, bf16), 2 / 4 / 8 53.9 / 57.4 / 57.3 us for both passes
 # (4096 x 2048, f32).
 CONV_UNITS, CONV_GRAD_UNITS = 8, 2
-# Blocks a multiprocessor of the norm: 2 / 4 / 6 / 16 70 / 71 / 77 / 80 us (8192 x 4096 bf16), backward 1 / 2 / 4 142 / 152 /
-# 170 us for both passes (4096 x 4096 bf16): every block sums its own share of the parameter gradients.
+# Blocks a multiprocessor of the norm: 2 / 4 / 6 / 16 68 / 70 / 76 / 79 us (8192 x 4096 bf16), backward 1 / 2 / 4 129 / 139 /
+# 155 us for both passes (4096 x 4096 bf16): every block sums its own share of the parameter gradients.
 NORM_UNITS, NORM_GRAD_UNITS = 2, 1
-# Sequences of at most this many rows go through the scan's token kernel.  4096 channels x 16 states, token kernel / walk:
-# 1 row 4.7 / 6.0 us (one sequence) and 26 / 73 us (128 sequences), 2 rows 6.0 / 6.0 and 41 / 75, 4 rows 8.3 / 5.9 and 72 / 77.
+# Sequences of at most this many rows go through the scan's token kernel (all of a plan's, or none: one longer sequence
+# sends the tokens beside it through the walk).  4096 channels x 16 states, bf16, token kernel / walk: 1 row 3.7 / 6.0 us (one
+# sequence) and 29 / 84 us (128 sequences), 2 rows 5.0 / 6.0 and 43 / 85, 4 rows 7.5 / 6.0 and 72 / 86.
 TOKEN_ROWS = 2
 # Sequences up to this length are not split; a unit has at least SCAN_LEAST_ROWS rows (512 rows x 1024 channels in units
-# of 32 / 64 / 128: 20 / 24 / 37 us), and a split makes about SCAN_BLOCKS blocks (16384 x 1024: 592 / 1184 / 2368 220 / 212 / 214 us).
+# of 32 / 64 / 128: 20 / 24 / 38 us), and a split makes about SCAN_BLOCKS blocks (16384 x 1024: 592 / 1184 / 2368 221 / 211 / 209 us).
 SCAN_WHOLE_ROWS, SCAN_LEAST_ROWS, SCAN_BLOCKS = 96, 32, 148 * 8
 
 
@@ -405,8 +406,8 @@ def _scan_units(a, args, tiles, row, work, twice):
     sequence takes ``row`` us a row however few blocks there are, and the whole batch ``work`` us a row and tile of
     channels.  Split, the batch takes ``twice`` that (every row's decay is computed again for the units' ends) and
     three launches.  The cheaper one is taken; measured on a B200, 4096 channels x 16 states, float32, unsplit / split:
-    2 x 1024 rows 147 / 119 us, 4 x 1024 178 / 217, 2 x 2048 289 / 221, 8 x 512 140 / 229; backward, 2048
-    channels: 2 x 512 rows 283 / 117, 8 x 256 188 / 214.  Returns the sequences' first units and what to place."""
+    2 x 1024 rows 143 / 117 us, 4 x 1024 174 / 214, 2 x 2048 280 / 216, 8 x 512 138 / 227; backward, 2048
+    channels: 2 x 512 rows 153 / 93, 8 x 256 151 / 168.  Returns the sequences' first units and what to place."""
     longest, total = max(int(a.lengths.max()), 1), int(a.lengths.sum())
     args.unit_rows = -(-longest // 32) * 32
     whole = max(longest * row, total * tiles * work)

