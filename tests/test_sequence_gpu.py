@@ -909,6 +909,63 @@ def test_graph_replay_steps_the_state(queue, rng):
     assert np.array_equal(s.state.buf.get(), want[0]) and np.array_equal(s.y.buf.get(), want[1])
 
 
+@pytest.mark.parametrize("lengths", [[300, 1, 0, 1, 40], [200, 180]], ids=str)
+def test_split_sequences_in_place_replayed(queue, rng, lengths):
+    """A prompt among single tokens, split over time, states in place: replays of a captured graph are launches of it."""
+    s = Scan(queue, rng, lengths, 40, 16, 1, BF16)
+    start = s.state.buf.get()
+    plan = s.plan(new_state=s.state.ra)
+    assert plan.full_args[0].n_units > len(lengths) and not plan.full_args[0].tokens
+    plan()
+    for k, end in enumerate(s.state.get()):
+        close(end, S.selective_scan(**s.of(k))[1], S.selective_scan(**s.of(k), magnitude=True)[1], s.chain(k), F32, "state")
+    for _ in range(3):
+        plan()
+    end = s.state.buf.get(), s.y.buf.get()
+    s.state.buf.set(start)
+    Plans([plan], False, unroll=2).call_n_times(4)
+    assert np.array_equal(s.state.buf.get(), end[0]) and np.array_equal(s.y.buf.get(), end[1])
+
+
+def test_training_pass_in_a_torch_graph(ctx, queue, rng):
+    """Forward and backward plans of all three operators captured by torch on its own stream, replayed twice while the
+    same plans also ran outside of it."""
+    torch = pytest.importorskip("torch")
+    side = torch.cuda.Stream()
+    q = CommandQueue(ctx, stream=side.cuda_stream)
+    lengths, chan = [70, 0, 33], 48
+    s = Scan(q, rng, lengths, chan, 16, 2, F32)
+    rows = lambda: Rows(q, [normal(rng, k, chan) for k in lengths], F32, columns=chan)
+    dy, outs = rows(), [Rows(q, v.values, F32, empty=True, columns=v.place[0][2]) for v in (s.x, s.dt, s.B, s.C)]
+    par = lambda *shape: vec(q, np.zeros(shape))
+    fwd = s.plan(keep=True)
+    plans = [fwd, seq.plan_selective_scan_grad(q, fwd, dy.ra, outs[0].ra, outs[1].ra, par(chan, 16), outs[2].ra, outs[3].ra)]
+    conv = seq.plan_causal_conv(q, s.x.ra, vec(q, normal(rng, chan, 4)), rows().ra, activation="silu")
+    cdx, cdw = rows(), par(chan, 4)
+    plans += [conv, seq.plan_causal_conv_grad(q, conv, dy.ra, cdx.ra, cdw)]
+    norm = seq.plan_residual_norm(q, s.x.ra, H=rows().ra, gate=s.z.ra, weight=vec(q, np.ones(chan)), groups=3)
+    ndx, ndw = rows(), par(chan)
+    plans += [norm, seq.plan_residual_norm_grad(q, norm, ndx.ra, dH=dy.ra, dweight=ndw)]
+    results = lambda: [r.buf.get() for r in outs + [s.y, cdx, ndx]] + [cdw.get(), ndw.get()]
+    for p in plans:
+        p.enqueue()
+    want = results()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        for p in plans:
+            p.enqueue()
+    for r in outs + [s.y, cdx, ndx]:
+        r.buf.set(np.full(r.buf.size, -7.5, np.float32))
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(np.array_equal(a, b) for a, b in zip(results(), want))
+        for p in plans:
+            p.enqueue()
+        assert all(np.array_equal(a, b) for a, b in zip(results(), want))
+
+
 def test_training_pass_replayed_and_on_another_stream(ctx, queue, rng):
     s = Scan(queue, rng, [70, 33], 40, 16, 2, F32)
     dy = Rows(queue, [normal(rng, k, 40) for k in s.lengths], F32)
